@@ -1,0 +1,294 @@
+"""Attention over a paged key-value cache on torch CUDA tensors (the amoe_rope_*, amoe_kv_*
+and amoe_attn_* entry points of include/amoe.h).
+
+The operators of the GPT-OSS layer's attention half between its two projections
+(internal/model/gptoss/layer.go:40-92, internal/backend/cpuref/attention.go:11-171,
+rope.go:10-86).  A serving loop holds one ``KVCache`` a layer, all over one page table:
+
+    rope = Rope(64, 150000.0)
+    cache = KVCache(pages, 64, kv_heads=8, head_dim=64, dtype=torch.float8_e4m3fn)
+    # a prompt: packed rows of all sequences, cu their starts
+    q = cache.append(k, v, table, past, cu, q=q, rope=rope, k_out=kr)   # kr: the rotated keys
+    out = prefill(q, kr, v, cu, window=128, sinks=sinks)
+    # a later chunk of the prompt reads what came before it back
+    k_all, v_all = cache.read(table, cu_k, total, dtype=torch.bfloat16)
+    # then one token a sequence and step
+    q = cache.append(k, v, table, length, cu, q=q, rope=rope)
+    out = cache.decode(q, table, length + 1, window=128, sinks=sinks)
+
+Work is enqueued on ``stream`` (default: torch's current stream on the tensors' device) and
+nothing waits for it.  Inputs, outputs and the cache must be ready on that stream, as with
+any torch operation.  Rows may be strided views with adjacent elements whose strides and
+address are multiples of 16 bytes (a fused projection's slices are).  Arguments that cannot
+be served raise ``AmoeError``; wrong page ids and lengths, which only the device sees, are
+skipped there and reported by ``KVCache.check``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .moe import (AMOE_ERR_INVALID, AMOE_OK, GGUF_BF16, GGUF_F16, GGUF_F32, KV_BAD_LENGTHS, KV_BAD_PAGE, KV_E4M3,
+                  KV_PAST_TABLE, AmoeAttn, AmoeError, AmoeKvCache, AmoeKvSeqs, AmoeRope, AmoeRows, load_library)
+
+_TYPES = {torch.float32: GGUF_F32, torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16}
+_CACHE_TYPES = {torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16, torch.float8_e4m3fn: KV_E4M3}
+
+
+def _invalid(message: str):
+    raise AmoeError(AMOE_ERR_INVALID, message)
+
+
+def _check(lib, rc: int):
+    if rc != AMOE_OK:
+        raise AmoeError(rc, lib.amoe_last_error(None).decode())
+
+
+def _rows(t, name: str, tokens: int, head_dim: int, device) -> AmoeRows:
+    """A [tokens, heads, head_dim] tensor as the C ABI's rows."""
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != head_dim:
+        _invalid(f"{name} must be [{tokens}, heads, {head_dim}], got {list(t.shape)}")
+    if t.device != device:
+        _invalid(f"{name} is on {t.device}, want {device}")
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        _invalid(f"{name} has type {t.dtype}")
+    st, sh, sd = t.stride()
+    if sd != 1:
+        _invalid(f"{name}: the elements of a row must be adjacent")
+    # a call without rows has no address to give
+    return AmoeRows(t.data_ptr() or 16, st, sh, t.shape[1], kind)
+
+
+def _written(t, name: str):
+    """Rows that a call writes must not share memory with one another."""
+    n, h, d = t.shape
+    st, sh, _ = t.stride()
+    if (n > 1 and st < d) or (h > 1 and sh < d) or (n > 1 and h > 1 and min(st, sh) * ((h if sh <= st else n) - 1) + d
+                                                   > max(st, sh)):
+        _invalid(f"{name}: its rows overlap")
+
+
+def _ints(t, name: str, n: int, device) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _invalid(f"{name} must be {n} adjacent int32 values")
+    if t.device != device:
+        _invalid(f"{name} is on {t.device}, want {device}")
+    return t.data_ptr()
+
+
+def _stream(stream, device):
+    """(the raw stream, a torch stream to allocate under or None for the current one)."""
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream, None
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    if stream.device != device:
+        _invalid(f"stream is on {stream.device}, want {device}")
+    return stream.cuda_stream, stream
+
+
+def _empty(shape, dtype, device, stream):
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _attn(scale, window: int, sinks, heads: int, device) -> AmoeAttn:
+    if scale is not None and not scale > 0:
+        _invalid("scale must be positive")
+    at = None
+    if sinks is not None:
+        if sinks.dtype != torch.float32 or sinks.dim() != 1 or sinks.shape[0] != heads or not sinks.is_contiguous():
+            _invalid(f"sinks must be {heads} adjacent float32 values")
+        if sinks.device != device:
+            _invalid(f"sinks is on {sinks.device}, want {device}")
+        at = sinks.data_ptr()
+    return AmoeAttn(scale or 0.0, window, at)
+
+
+class Rope:
+    """Rotary frequencies (RoPE, or GPT-OSS's YaRN: rope.go:10-44)."""
+
+    def __init__(self, head_dim: int, theta: float = 150000.0, yarn: bool = True):
+        lib = load_library()
+        self._c = AmoeRope()
+        _check(lib, lib.amoe_rope_init(head_dim, theta, 1 if yarn else 0, ctypes.byref(self._c)))
+
+    @property
+    def frequencies(self) -> list:
+        return list(self._c.freq)[:self._c.head_dim // 2]
+
+    @property
+    def concentration(self) -> float:
+        return self._c.concentration
+
+
+class KVCache:
+    """One layer's paged cache: ``k`` and ``v`` [pages, kv_heads, page_size, head_dim] in float16,
+    bfloat16 or float8_e4m3fn, the last with one E8M0 byte for each token and head in
+    ``k_scale`` and ``v_scale`` [pages, kv_heads, page_size].  Calls take the page table
+    [seqs, n] (int32; row s lists sequence s's pages in order)."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,
+                 device="cuda"):
+        shape = (pages, kv_heads, page_size, head_dim)
+        if min(shape) < 1:
+            _invalid(f"a cache of shape {shape}")
+        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        ks = vs = None
+        if dtype == torch.float8_e4m3fn:
+            ks, vs = (torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2))
+        self._set(k, v, ks, vs)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale=None, v_scale=None) -> "KVCache":
+        """A cache over pages that the caller holds."""
+        self = cls.__new__(cls)
+        self._set(k, v, k_scale, v_scale)
+        return self
+
+    def _set(self, k, v, k_scale, v_scale):
+        kind = _CACHE_TYPES.get(k.dtype)
+        if kind is None or v.dtype != k.dtype:
+            _invalid(f"a cache of {k.dtype} and {v.dtype}: float16, bfloat16 or float8_e4m3fn")
+        if k.dim() != 4 or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous():
+            _invalid("cache pages must be [pages, kv_heads, page_size, head_dim], contiguous, alike for k and v")
+        if not k.is_cuda or v.device != k.device:
+            _invalid("cache pages must be on one CUDA device")
+        if any((s is not None) != (kind == KV_E4M3) for s in (k_scale, v_scale)):
+            _invalid("k_scale and v_scale go with an E4M3 cache, and with no other")
+        for s in (k_scale, v_scale):
+            if s is not None and (s.dtype != torch.uint8 or s.shape != k.shape[:3] or not s.is_contiguous()
+                                  or s.device != k.device):
+                _invalid("scales must be uint8 [pages, kv_heads, page_size] beside the pages")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.device
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._lib = load_library()
+        self._c = AmoeKvCache(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
+                              None if v_scale is None else v_scale.data_ptr(), self.status.data_ptr(), self.pages,
+                              self.page_size, self.kv_heads, self.head_dim, kind, k.device.index)
+
+    def _seqs(self, page_table) -> AmoeKvSeqs:
+        t = page_table
+        if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.device != self.device:
+            _invalid(f"page_table must be int32 [seqs, pages] with adjacent columns on {self.device}")
+        if t.shape[0] < 1 or t.shape[1] < 1 or (t.shape[0] > 1 and t.stride(0) != t.shape[1]):
+            _invalid("page_table must be contiguous and not empty")
+        return AmoeKvSeqs(t.data_ptr(), t.shape[1], t.shape[0])
+
+    def append(self, k, v, page_table, past, cu, q=None, rope: Rope | None = None, q_type=None, q_out=None,
+               k_out=None, v_out=None, stream=None):
+        """Rotates and writes packed new rows (amoe_kv_append): rows cu[s]..cu[s+1] of k and v
+        [tokens, kv_heads, head_dim] become sequence s's tokens past[s], past[s] + 1, ...
+        Returns the rotated q [tokens, q_heads, head_dim] (``q_out``, or a new tensor of
+        ``q_type``, by default q's own), None without q."""
+        n, dev = k.shape[0], self.device
+        seqs = self._seqs(page_table)
+        raw, st = _stream(stream, dev)
+        ck, cv = _rows(k, "k", n, self.head_dim, dev), _rows(v, "v", n, self.head_dim, dev)
+        cq = cqo = cko = cvo = None
+        if q is not None:
+            cq = _rows(q, "q", n, self.head_dim, dev)
+            if q_out is None:
+                q_out = _empty(q.shape, q_type or q.dtype, dev, st)
+            elif q_type is not None and q_out.dtype != q_type:
+                _invalid(f"q_out is {q_out.dtype}, q_type {q_type}")
+        elif q_out is not None:
+            _invalid("q_out without q")
+        if q_out is not None:
+            _written(q_out, "q_out")
+            cqo = ctypes.byref(_rows(q_out, "q_out", n, self.head_dim, dev))
+        if k_out is not None:
+            _written(k_out, "k_out")
+            cko = ctypes.byref(_rows(k_out, "k_out", n, self.head_dim, dev))
+        if v_out is not None:
+            _written(v_out, "v_out")
+            cvo = ctypes.byref(_rows(v_out, "v_out", n, self.head_dim, dev))
+        _check(self._lib, self._lib.amoe_kv_append(
+            ctypes.byref(self._c), ctypes.byref(seqs), _ints(cu, "cu", seqs.seqs + 1, dev),
+            _ints(past, "past", seqs.seqs, dev), n, None if rope is None else ctypes.byref(rope._c),
+            None if cq is None else ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv), cqo, cko, cvo, raw))
+        return q_out
+
+    def read(self, page_table, cu, total: int, dtype=None, first=None, k_out=None, v_out=None, stream=None):
+        """Sequence s's keys and values from position first[s] (default 0) on as packed rows
+        cu[s]..cu[s+1] (amoe_kv_read).  Returns (k, v) [total, kv_heads, head_dim]: k_out and v_out,
+        or new tensors of ``dtype`` (default: the cache's own type, bfloat16 for E4M3)."""
+        dev = self.device
+        seqs = self._seqs(page_table)
+        raw, st = _stream(stream, dev)
+        if dtype is None:
+            dtype = torch.bfloat16 if self._c.type == KV_E4M3 else self.k.dtype
+        shape = (total, self.kv_heads, self.head_dim)
+        k_out = _empty(shape, dtype, dev, st) if k_out is None else k_out
+        v_out = _empty(shape, dtype, dev, st) if v_out is None else v_out
+        _written(k_out, "k_out")
+        _written(v_out, "v_out")
+        ck = _rows(k_out, "k_out", total, self.head_dim, dev)
+        cv = _rows(v_out, "v_out", total, self.head_dim, dev)
+        _check(self._lib, self._lib.amoe_kv_read(
+            ctypes.byref(self._c), ctypes.byref(seqs), _ints(cu, "cu", seqs.seqs + 1, dev),
+            None if first is None else _ints(first, "first", seqs.seqs, dev), total, ctypes.byref(ck),
+            ctypes.byref(cv), raw))
+        return k_out, v_out
+
+    def decode(self, q, page_table, kv_len, scale: float | None = None, window: int = 0, sinks=None,
+               max_len: int = 0, out=None, stream=None):
+        """Attention of one new token a sequence (amoe_attn_decode): q [seqs, q_heads, head_dim] at
+        position kv_len[s] - 1.  Returns out, like q."""
+        dev = self.device
+        seqs = self._seqs(page_table)
+        raw, st = _stream(stream, dev)
+        cq = _rows(q, "q", seqs.seqs, self.head_dim, dev)
+        if out is None:
+            out = _empty(q.shape, q.dtype, dev, st)
+        else:
+            _written(out, "out")
+        co = _rows(out, "out", seqs.seqs, self.head_dim, dev)
+        attn = _attn(scale, window, sinks, q.shape[1], dev)
+        _check(self._lib, self._lib.amoe_attn_decode(
+            ctypes.byref(self._c), ctypes.byref(seqs), ctypes.byref(attn), ctypes.byref(cq), ctypes.byref(co),
+            _ints(kv_len, "kv_len", seqs.seqs, dev), max_len, raw))
+        return out
+
+    def check(self):
+        """Waits for the device and raises if a call met a wrong page id or length since the last check."""
+        bits = int(self.status.item())
+        if not bits:
+            return
+        self.status.zero_()
+        said = [m for b, m in ((KV_BAD_PAGE, "a page id outside the cache"),
+                               (KV_PAST_TABLE, "a position beyond the page table"),
+                               (KV_BAD_LENGTHS, "negative or decreasing lengths")) if bits & b]
+        _invalid("kv cache: " + ", ".join(said))
+
+
+def prefill(q, k, v, cu_q, cu_k=None, scale: float | None = None, window: int = 0, sinks=None, out=None,
+            stream=None):
+    """Causal attention of packed prompts (amoe_attn_prefill): rows cu_q[s]..cu_q[s+1] of q
+    [tokens, q_heads, head_dim] are the last of the positions that rows cu_k[s]..cu_k[s+1] of
+    k and v [keys, kv_heads, head_dim] hold (cu_k None: cu_q).  Returns out, like q."""
+    lib = load_library()
+    dev = q.device
+    if not q.is_cuda or q.dim() != 3:
+        _invalid("q must be a CUDA tensor [tokens, q_heads, head_dim]")
+    cu_k = cu_q if cu_k is None else cu_k
+    seqs = cu_q.shape[0] - 1
+    raw, st = _stream(stream, dev)
+    n, m, d = q.shape[0], k.shape[0], q.shape[2]
+    if out is None:
+        out = _empty(q.shape, q.dtype, dev, st)
+    else:
+        _written(out, "out")
+    cq, co = _rows(q, "q", n, d, dev), _rows(out, "out", n, d, dev)
+    ck, cv = _rows(k, "k", m, d, dev), _rows(v, "v", m, d, dev)
+    attn = _attn(scale, window, sinks, q.shape[1], dev)
+    _check(lib, lib.amoe_attn_prefill(
+        dev.index, d, ctypes.byref(attn), ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv), ctypes.byref(co),
+        n, m, _ints(cu_q, "cu_q", seqs + 1, dev), _ints(cu_k, "cu_k", seqs + 1, dev), seqs, raw))
+    return out

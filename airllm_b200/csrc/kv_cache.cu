@@ -1,0 +1,357 @@
+// kv_cache.cu -- the paged key-value cache's writes and reads: rotation, quantisation and
+// append (yarnHeads, internal/model/gptoss/layer.go:189-207; YaRNRoPE,
+// internal/backend/cpuref/rope.go:17-86; KVCache.Append, attention.go:40-59), and the gather
+// of a sequence's pages back into packed rows.
+//
+// append.  Element i and i + d/2 of a head turn by the angle pos * freq[i]:
+//   y[i] = x[i] c - x[i + d/2] s,  y[i + d/2] = x[i + d/2] c + x[i] s,
+// c and s = cos, sin (angle) * concentration.  Angles of far positions lose float32, and a
+// value that lands next to a rounding border of the cache's type must fall on the side the
+// definition says, so angles, sines and products are float64 as in the reference, rounded
+// once to float32 (its stored type) and from there to the cache's.  One CTA takes one token:
+// d/2 threads compute the angles, then d/16 threads a head row turn eight pairs each with
+// the sines of their eight pairs in registers for every row they visit.
+//
+// E4M3 rows: the scale is a power of two, so scaling is exact and only the rounding to E4M3
+// loses bits; the row's maximum is reduced over the d/16 lanes that hold it.
+#include "attn.cuh"
+
+namespace amoe {
+namespace attn {
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kReadThreads = 256;
+constexpr int kReadTokens = 16;
+constexpr int kNoRow = INT_MIN;  // in the place of a page: not a row of this call
+
+struct RopeDev {
+    double freq[AMOE_ROPE_MAX_HALF];
+    double conc;
+    int on;
+};
+
+struct AppendParams {
+    CacheDev c;
+    RowsDev q, k, v, q_out, k_out, v_out;
+    const int32_t *cu, *past;
+    int tokens, seqs, q_heads, q_out_type, k_out_type, v_out_type;
+    RopeDev rope;
+};
+
+// Smallest e with amax <= 448 * 2^e, at least -127; 0 for amax == 0.  amax = 1.f * 2^(E - 127)
+// and 448 * 2^e = 1.75 * 2^(e + 8).
+__device__ __forceinline__ int e4m3_exp(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    if (b == 0u) return 0;
+    const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -127 ? -127 : e;
+}
+
+// 2^e, e in [-127, 127].
+__device__ __forceinline__ float exp2i(int e) {
+    return e == -127 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n .reg .b16 t;\n cvt.rn.satfinite.e4m3x2.f32 t, %1, %2;\n cvt.u32.u16 %0, t;\n}"
+        : "=r"(r)
+        : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint2 e4m3x8(const float (&x)[8], float by) {
+    return make_uint2(e4m3x2(x[0] * by, x[1] * by) | e4m3x2(x[2] * by, x[3] * by) << 16,
+                      e4m3x2(x[4] * by, x[5] * by) | e4m3x2(x[6] * by, x[7] * by) << 16);
+}
+
+// One thread's two groups of eight (elements i0.. and i0 + D/2..) of one row into the cache.
+// All D/16 lanes of the row call it together.
+template <int D, int CACHE>
+__device__ __forceinline__ void cache_store(char *pages, uint8_t *scales, int64_t row, int part, const float (&a)[8],
+                                            const float (&b)[8], bool write) {
+    if constexpr (CACHE == AMOE_KV_E4M3) {
+        float amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            amax = fmaxf(amax, fmaxf(fabsf(a[i]), fabsf(b[i])));
+            bad |= !isfinite(a[i]) || !isfinite(b[i]);
+        }
+        if (bad) amax = INFINITY;
+#pragma unroll
+        for (int m = 1; m < D / 16; m <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+        if (!write) return;
+        char *dst = pages + row * D + part * 8;
+        if (amax == INFINITY) {
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+            *reinterpret_cast<uint2 *>(dst + D / 2) = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+            if (part == 0) scales[row] = 255;
+            return;
+        }
+        const int e = e4m3_exp(amax);
+        const float by = exp2i(-e);
+        *reinterpret_cast<uint2 *>(dst) = e4m3x8(a, by);
+        *reinterpret_cast<uint2 *>(dst + D / 2) = e4m3x8(b, by);
+        if (part == 0) scales[row] = (uint8_t)(e + 127);
+    } else {
+        if (!write) return;
+        char *dst = pages + (row * D + part * 8) * 2;
+        store8<CACHE>(dst, a);
+        store8<CACHE>(dst + D, b);
+    }
+}
+
+template <int D, int SRC, int CACHE>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
+    constexpr int L = D / 16;  // lanes of a row
+    constexpr int ES = SRC == AMOE_GGUF_F32 ? 4 : 2;
+    __shared__ double2 cs[D / 2];
+    const int t = blockIdx.x;
+    const int last = p.cu[p.seqs];
+    if (t >= last) return;
+    const int s = find_seq(p.cu, p.seqs, t);
+    const int start = p.cu[s], past = p.past[s];
+    if (start > t || start < 0 || p.cu[s + 1] <= t || past < 0) {
+        if (threadIdx.x == 0) atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
+        return;
+    }
+    const int64_t pos = (int64_t)past + (t - start);
+    if (p.rope.on && threadIdx.x < D / 2) {
+        double sn, c;
+        sincos((double)pos * p.rope.freq[threadIdx.x], &sn, &c);
+        cs[threadIdx.x] = make_double2(c * p.rope.conc, sn * p.rope.conc);
+    }
+    const int page = page_of(p.c, s, pos);
+    __syncthreads();
+
+    const int part = threadIdx.x % L;
+    double2 w[8];
+    if (p.rope.on) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = cs[part * 8 + i];
+    }
+    const int rows = p.q_heads + 2 * p.c.heads;
+    // whole warps stay together for the row maximum's shuffles: the bound is rounded up
+    for (int r0 = 0; r0 < rows; r0 += kAppendThreads / L) {
+        const int r = r0 + threadIdx.x / L;
+        const bool live = r < rows;
+        const bool is_q = r < p.q_heads, is_k = !is_q && r < p.q_heads + p.c.heads;
+        const int h = is_q ? r : is_k ? r - p.q_heads : r - p.q_heads - p.c.heads;
+        float a[8] = {}, b[8] = {};
+        if (live) {
+            const RowsDev &src = is_q ? p.q : is_k ? p.k : p.v;
+            const char *x = src.p + t * src.ts + h * src.hs + part * 8 * ES;
+            load8<SRC>(x, a);
+            load8<SRC>(x + D / 2 * ES, b);
+            if (p.rope.on && (is_q || is_k)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const double f = a[i], g = b[i];
+                    a[i] = (float)(f * w[i].x - g * w[i].y);
+                    b[i] = (float)(g * w[i].x + f * w[i].y);
+                }
+            }
+            const RowsDev &dst = is_q ? p.q_out : is_k ? p.k_out : p.v_out;
+            if (dst.p) {
+                const int type = is_q ? p.q_out_type : is_k ? p.k_out_type : p.v_out_type;
+                const int es = elem_size(type);
+                char *y = dst.p + t * dst.ts + h * dst.hs + part * 8 * es;
+                store8_any(y, type, a);
+                store8_any(y + D / 2 * es, type, b);
+            }
+        }
+        const bool write = live && !is_q && page >= 0;
+        const int64_t row = write ? cache_row(p.c, page, h, pos) : 0;
+        cache_store<D, CACHE>(is_k ? p.c.k : p.c.v, is_k ? p.c.ks : p.c.vs, row, part, a, b, write);
+    }
+}
+
+struct ReadParams {
+    CacheDev c;
+    RowsDev k, v;
+    const int32_t *cu, *first;
+    int tokens, seqs, k_type, v_type;
+};
+
+template <int D, int CACHE>
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ ReadParams p) {
+    constexpr int C = D / 8;  // eight elements an item
+    __shared__ int page[kReadTokens];
+    __shared__ int64_t pos[kReadTokens];
+    const int t0 = blockIdx.x * kReadTokens;
+    const int last = min(p.cu[p.seqs], p.tokens);
+    if (t0 >= last) return;
+    if (threadIdx.x < kReadTokens) {
+        const int t = t0 + threadIdx.x;
+        int pg = kNoRow;
+        int64_t at = 0;
+        if (t < last) {
+            const int s = find_seq(p.cu, p.seqs, t);
+            const int start = p.cu[s];
+            const int64_t f = p.first ? p.first[s] : 0;
+            if (start < 0 || start > t || p.cu[s + 1] <= t || f < 0) {
+                atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
+            } else {
+                at = f + (t - start);
+                pg = page_of(p.c, s, at);
+            }
+        }
+        page[threadIdx.x] = pg;
+        pos[threadIdx.x] = at;
+    }
+    __syncthreads();
+    const int per = p.c.heads * C;  // items of one token's keys or values
+    for (int i = threadIdx.x; i < kReadTokens * 2 * per; i += kReadThreads) {
+        const int tok = i / (2 * per), j = i % (2 * per);
+        const bool is_v = j >= per;
+        const int h = (j % per) / C, ch = j % C;
+        const int pg = page[tok];
+        if (pg == kNoRow) continue;
+        float x[8] = {};
+        if (pg >= 0) {
+            const int64_t row = cache_row(p.c, pg, h, pos[tok]);
+            const char *src = is_v ? p.c.v : p.c.k;
+            if constexpr (CACHE == AMOE_KV_E4M3) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(src + row * D + ch * 8);
+                const float by = e8m0_to_float((is_v ? p.c.vs : p.c.ks)[row]);
+                const uint32_t u[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const uint32_t hh = e4m3x2_to_f16x2(u[m]);
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hh));
+                    x[2 * m] = f.x * by, x[2 * m + 1] = f.y * by;
+                }
+            } else {
+                load8<CACHE>(src + (row * D + ch * 8) * 2, x);
+            }
+        }
+        const RowsDev &dst = is_v ? p.v : p.k;
+        const int type = is_v ? p.v_type : p.k_type;
+        store8_any(dst.p + (int64_t)(t0 + tok) * dst.ts + h * dst.hs + ch * 8 * elem_size(type), type, x);
+    }
+}
+
+template <int D, int SRC>
+cudaError_t launch_append(const AppendParams &p, int cache, cudaStream_t st) {
+    if (cache == AMOE_GGUF_F16) append_kernel<D, SRC, AMOE_GGUF_F16><<<p.tokens, kAppendThreads, 0, st>>>(p);
+    else if (cache == AMOE_GGUF_BF16) append_kernel<D, SRC, AMOE_GGUF_BF16><<<p.tokens, kAppendThreads, 0, st>>>(p);
+    else append_kernel<D, SRC, AMOE_KV_E4M3><<<p.tokens, kAppendThreads, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_append_d(const AppendParams &p, int src, int cache, cudaStream_t st) {
+    if (src == AMOE_GGUF_F32) return launch_append<D, AMOE_GGUF_F32>(p, cache, st);
+    if (src == AMOE_GGUF_F16) return launch_append<D, AMOE_GGUF_F16>(p, cache, st);
+    return launch_append<D, AMOE_GGUF_BF16>(p, cache, st);
+}
+
+template <int D>
+cudaError_t launch_read_d(const ReadParams &p, int cache, cudaStream_t st) {
+    const int grid = (p.tokens - 1) / kReadTokens + 1;
+    if (cache == AMOE_GGUF_F16) read_kernel<D, AMOE_GGUF_F16><<<grid, kReadThreads, 0, st>>>(p);
+    else if (cache == AMOE_GGUF_BF16) read_kernel<D, AMOE_GGUF_BF16><<<grid, kReadThreads, 0, st>>>(p);
+    else read_kernel<D, AMOE_KV_E4M3><<<grid, kReadThreads, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace amoe
+
+using namespace amoe;
+using namespace amoe::attn;
+
+extern "C" {
+
+int amoe_rope_init(int32_t head_dim, double theta, int32_t yarn, amoe_rope *out) {
+    if (!out) return reject("out must not be NULL");
+    if (head_dim <= 0 || head_dim % 2) return reject("rope head dimension must be positive and even");
+    if (head_dim > 2 * AMOE_ROPE_MAX_HALF)
+        return reject("rope head dimension above " + std::to_string(2 * AMOE_ROPE_MAX_HALF));
+    if (!(theta > 0) || std::isinf(theta)) return reject("rope theta must be finite and positive");
+    *out = {};
+    const int half = head_dim / 2;
+    const double factor = 32.0, original = 4096.0, pi = 3.14159265358979323846;
+    auto corner = [&](double beta) { return head_dim * std::log(original / (beta * 2.0 * pi)) / (2.0 * std::log(theta)); };
+    const double low = std::fmax(0.0, std::floor(corner(32.0)));
+    const double high = std::fmin(half - 1.0, std::ceil(corner(1.0)));
+    for (int i = 0; i < half; ++i) {
+        out->freq[i] = std::pow(theta, -2.0 * i / head_dim);
+        if (!yarn) continue;
+        const double ramp = high == low ? 0.0 : std::fmax(0.0, std::fmin(1.0, (i - low) / (high - low)));
+        out->freq[i] *= ramp + (1.0 - ramp) / factor;
+    }
+    out->concentration = yarn ? 1.0 + 0.1 * std::log(factor) : 1.0;
+    out->head_dim = head_dim;
+    return AMOE_OK;
+}
+
+int amoe_kv_append(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const int32_t *cu, const int32_t *past,
+                   int32_t tokens, const amoe_rope *rope, const amoe_rows *q, const amoe_rows *k, const amoe_rows *v,
+                   const amoe_rows *q_out, const amoe_rows *k_out, const amoe_rows *v_out, void *stream) {
+    if (int rc = check_cache(cache, seqs)) return rc;
+    if (!cu || !past) return reject("cu and past must not be NULL");
+    if (tokens < 0) return reject("tokens must not be negative");
+    const int D = cache->head_dim, kv = cache->kv_heads;
+    if (int rc = check_rows(k, "k", D, kv, tokens, -1)) return rc;
+    if (int rc = check_rows(v, "v", D, kv, tokens, k->type)) return rc;
+    if (q)
+        if (int rc = check_rows(q, "q", D, 0, tokens, k->type)) return rc;
+    if (q_out && !q) return reject("q_out without q");
+    if (q_out)
+        if (int rc = check_rows(q_out, "q_out", D, q->heads, tokens, -1)) return rc;
+    if (k_out)
+        if (int rc = check_rows(k_out, "k_out", D, kv, tokens, -1)) return rc;
+    if (v_out)
+        if (int rc = check_rows(v_out, "v_out", D, kv, tokens, -1)) return rc;
+    if (rope && rope->head_dim != D) return reject("the rope's head_dim differs from the cache's");
+    if (tokens == 0) return AMOE_OK;
+    AppendParams p{};
+    p.c = cache_dev(cache, seqs);
+    p.q = rows_dev(q), p.k = rows_dev(k), p.v = rows_dev(v);
+    p.q_out = rows_dev(q_out), p.k_out = rows_dev(k_out), p.v_out = rows_dev(v_out);
+    p.cu = cu, p.past = past;
+    p.tokens = tokens, p.seqs = seqs->seqs;
+    p.q_heads = q && q_out ? q->heads : 0;  // a q that goes nowhere is not read
+    p.q_out_type = q_out ? q_out->type : 0;
+    p.k_out_type = k_out ? k_out->type : 0;
+    p.v_out_type = v_out ? v_out->type : 0;
+    if (rope) {
+        for (int i = 0; i < D / 2; ++i) p.rope.freq[i] = rope->freq[i];
+        p.rope.conc = rope->concentration;
+        p.rope.on = 1;
+    }
+    DeviceScope scope;
+    cudaError_t e = scope.enter(cache->device);
+    if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    e = D == 64 ? launch_append_d<64>(p, k->type, cache->type, st) : launch_append_d<128>(p, k->type, cache->type, st);
+    return e == cudaSuccess ? AMOE_OK : cuda_error(e, "append kernel");
+}
+
+int amoe_kv_read(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const int32_t *cu, const int32_t *first,
+                 int32_t tokens, const amoe_rows *k_out, const amoe_rows *v_out, void *stream) {
+    if (int rc = check_cache(cache, seqs)) return rc;
+    if (!cu) return reject("cu must not be NULL");
+    if (tokens < 0) return reject("tokens must not be negative");
+    if (int rc = check_rows(k_out, "k_out", cache->head_dim, cache->kv_heads, tokens, -1)) return rc;
+    if (int rc = check_rows(v_out, "v_out", cache->head_dim, cache->kv_heads, tokens, -1)) return rc;
+    if (tokens == 0) return AMOE_OK;
+    ReadParams p{};
+    p.c = cache_dev(cache, seqs);
+    p.k = rows_dev(k_out), p.v = rows_dev(v_out);
+    p.cu = cu, p.first = first;
+    p.tokens = tokens, p.seqs = seqs->seqs;
+    p.k_type = k_out->type, p.v_type = v_out->type;
+    DeviceScope scope;
+    cudaError_t e = scope.enter(cache->device);
+    if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    e = cache->head_dim == 64 ? launch_read_d<64>(p, cache->type, st) : launch_read_d<128>(p, cache->type, st);
+    return e == cudaSuccess ? AMOE_OK : cuda_error(e, "read kernel");
+}
+
+}  // extern "C"

@@ -52,6 +52,29 @@ class AmoeConfig(ctypes.Structure):
     ]
 
 
+class AmoeRows(ctypes.Structure):
+    _fields_ = [("data", _vp), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("heads", _i32),
+                ("type", _i32)]
+
+
+class AmoeKvCache(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("status", _vp),
+                ("pages", ctypes.c_int64), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("type", _i32), ("device", _i32)]
+
+
+class AmoeKvSeqs(ctypes.Structure):
+    _fields_ = [("page_table", _vp), ("table_stride", _i32), ("seqs", _i32)]
+
+
+class AmoeRope(ctypes.Structure):
+    _fields_ = [("freq", ctypes.c_double * 64), ("concentration", ctypes.c_double), ("head_dim", _i32)]
+
+
+class AmoeAttn(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("window", _i32), ("sinks", _vp)]
+
+
 AMOE_STAGES = 8
 STAGE_NAMES = ["route", "scan", "gate_up", "down", "combine", "scatter_gather", "decode_experts", "reserved7"]
 
@@ -98,9 +121,16 @@ SIGNATURES = {
     "amoe_head_upload_gguf": (ctypes.c_int, [_vp, _vp]),
     "amoe_head_next_token": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp]),
     "amoe_head_next_token_device": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp, _vp]),
+    "amoe_rope_init": (ctypes.c_int, [_i32, ctypes.c_double, _i32, _vp]),
+    "amoe_kv_append": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "amoe_kv_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "amoe_attn_prefill": (ctypes.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "amoe_attn_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp]),
 }
 
 GGUF_F32, GGUF_F16, GGUF_BF16, GGUF_MXFP4 = 0, 1, 30, 39
+KV_E4M3 = 100
+KV_BAD_PAGE, KV_PAST_TABLE, KV_BAD_LENGTHS = 1, 2, 4  # amoe_kv_cache.status
 
 _lib = None
 

@@ -306,6 +306,124 @@ AMOE_API int amoe_head_next_token(amoe_head *h, const float *hidden, int32_t T, 
 AMOE_API int amoe_head_next_token_device(amoe_head *h, const float *hidden, int32_t T, int32_t *tokens,
                                          float *logits, void *stream);
 
+/* ---- attention over a paged key-value cache ------------------------------------------
+ * The operators of the layer's attention half (internal/model/gptoss/layer.go:40-92,
+ * internal/backend/cpuref/attention.go:11-171, rope.go:10-86) between its two projections:
+ * rotate and append, read back, attention of packed prompts, attention of one new token a
+ * sequence.  They work on caller-owned device memory, keep nothing between calls, allocate
+ * nothing and need no context; like amoe_route_noalloc they leave the calling thread's
+ * current device as it was, and report failures through amoe_last_error(NULL).  Every call
+ * is enqueued on `stream` (a cudaStream_t; NULL = the legacy default stream) and returns
+ * without synchronising; it may be captured into a graph, and calls on different streams
+ * may overlap as long as none writes what another reads or writes.
+ * Shapes: head_dim 64 or 128; query heads a multiple of kv_heads, at most 128 of them to
+ * one kv head.  Element types are AMOE_GGUF_F32, AMOE_GGUF_F16 and AMOE_GGUF_BF16. */
+
+/* Packed rows [tokens][heads][head_dim]: elements of a row adjacent, strides in elements.
+ * data and the strides must be multiples of 16 bytes.  Rows that a call writes must not
+ * overlap one another or its inputs. */
+typedef struct amoe_rows {
+    void *data;
+    int64_t token_stride, head_stride;
+    int32_t heads, type;
+} amoe_rows;
+
+/* Cache element type beside AMOE_GGUF_F16 and AMOE_GGUF_BF16: E4M3 codes with one E8M0
+ * scale for each (token, kv head), 2^(byte - 127).  The exponent e is the smallest with
+ * max|x| <= 448 * 2^e over the row (0 for a row of zeros, at least -127); codes round to
+ * nearest, ties to even.  A row that holds an infinity or NaN is stored as NaN (byte 255). */
+enum { AMOE_KV_E4M3 = 100 };
+
+/* What kernels add to *status when a page table or length is wrong; the rows concerned are
+ * not written (append), read as zeros (read) or not seen (decode). */
+enum {
+    AMOE_KV_BAD_PAGE = 1,    /* a page id outside [0, pages) */
+    AMOE_KV_PAST_TABLE = 2,  /* a position beyond table_stride * page_size */
+    AMOE_KV_BAD_LENGTHS = 4  /* a negative length, or starts that decrease or pass the rows given */
+};
+
+/* One layer's cache (KVCache, attention.go:11-59): pages of page_size tokens, page_size a
+ * power of two up to 4096.  k and v: [pages][kv_heads][page_size][head_dim] elements of
+ * `type`; k_scale and v_scale: [pages][kv_heads][page_size] bytes (E4M3, else NULL); 16-byte
+ * aligned.  status: one device word that the caller zeroes and reads.  A page may stand in
+ * several sequences' tables (a shared prefix) as long as no call appends to it. */
+typedef struct amoe_kv_cache {
+    void *k, *v;
+    uint8_t *k_scale, *v_scale;
+    int32_t *status;
+    int64_t pages;
+    int32_t page_size, kv_heads, head_dim, type, device;
+} amoe_kv_cache;
+
+/* The sequences of a call.  page_table [seqs][table_stride] page ids; token t of sequence s
+ * lies in page page_table[s][t / page_size] at slot t % page_size.  Device memory. */
+typedef struct amoe_kv_seqs {
+    const int32_t *page_table;
+    int32_t table_stride, seqs;
+} amoe_kv_seqs;
+
+/* Rotation of a head's two halves by position * freq (rope.go:10-86), scaled. */
+#define AMOE_ROPE_MAX_HALF 64
+typedef struct amoe_rope {
+    double freq[AMOE_ROPE_MAX_HALF];
+    double concentration;
+    int32_t head_dim;
+} amoe_rope;
+
+/* Replaces: the frequency tables of RoPE and YaRNRoPE (rope.go:10-44; yarn != 0: GPT-OSS's
+ * factor 32 over an original context of 4096).  No GPU needed.  head_dim even, 2..128. */
+AMOE_API int amoe_rope_init(int32_t head_dim, double theta, int32_t yarn, amoe_rope *out);
+
+/* Replaces: yarnHeads (layer.go:189-207) and KVCache.Append (attention.go:40-59).  Packed
+ * new tokens: rows cu[s] .. cu[s+1] - 1 of q, k and v (cu [seqs + 1], device) belong to
+ * sequence s and stand at positions past[s], past[s] + 1, ...  q and k are rotated there
+ * in float64 (rope NULL: left as they are) and rounded to float32, as the reference stores
+ * them; k and v then go into the cache, rounded to its type or quantised.  q_out, k_out and
+ * v_out (each nullable) receive the rotated q and k and the v in their own type (F32, F16
+ * or BF16), for a prefill of the same tokens; q may be NULL.  q, k and v have one type,
+ * `tokens` rows each; rows from cu[seqs] on are ignored. */
+AMOE_API int amoe_kv_append(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const int32_t *cu,
+                            const int32_t *past, int32_t tokens, const amoe_rope *rope, const amoe_rows *q,
+                            const amoe_rows *k, const amoe_rows *v, const amoe_rows *q_out,
+                            const amoe_rows *k_out, const amoe_rows *v_out, void *stream);
+
+/* Reads the cache back: rows cu[s] .. cu[s+1] - 1 of k_out and v_out receive the keys and
+ * values of sequence s from position first[s] on (first NULL: 0), in k_out's and v_out's
+ * type.  `tokens` rows each; rows from cu[seqs] on are left as they are. */
+AMOE_API int amoe_kv_read(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const int32_t *cu,
+                          const int32_t *first, int32_t tokens, const amoe_rows *k_out, const amoe_rows *v_out,
+                          void *stream);
+
+/* Scores are scale * q.k (scale 0: 1 / sqrt(head_dim)); window > 0: a query sees the last
+ * `window` keys up to its own position only; sinks [q heads] (device, nullable): a learned
+ * logit for each head that joins the softmax's denominator (attention.go:82-171).  A query
+ * that sees no key gives a row of zeros. */
+typedef struct amoe_attn {
+    float scale;
+    int32_t window;
+    const float *sinks;
+} amoe_attn;
+
+/* Replaces: CausalAttentionWithConfig (attention.go:82-171) for packed prompts: rows
+ * cu_q[s] .. cu_q[s+1] - 1 of q and out and cu_k[s] .. cu_k[s+1] - 1 of k and v are
+ * sequence s, whose queries are the last of its keys' positions; each sees the keys up to
+ * its own.  q, k, v and out have one type, F16 or BF16; products accumulate in float32 and
+ * the softmax's maximum and sum are float32, its weights rounded to that type.  q_tokens and
+ * k_tokens are the rows given; rows of out from cu_q[seqs] on are left as they are. */
+AMOE_API int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, const amoe_rows *q,
+                               const amoe_rows *k, const amoe_rows *v, const amoe_rows *out, int32_t q_tokens,
+                               int32_t k_tokens, const int32_t *cu_q, const int32_t *cu_k, int32_t seqs,
+                               void *stream);
+
+/* The same for one new token a sequence, over the cache: row s of q and out is the query at
+ * position kv_len[s] - 1 of sequence s (kv_len [seqs], device, the new token included; 0: a
+ * row of zeros).  q and out are F16 or BF16, the cache's type or any with an E4M3 cache.
+ * max_len bounds the lengths the call is laid out for (0: the table's capacity); longer
+ * ones give the same result in more time. */
+AMOE_API int amoe_attn_decode(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const amoe_attn *attn,
+                              const amoe_rows *q, const amoe_rows *out, const int32_t *kv_len, int32_t max_len,
+                              void *stream);
+
 /* ABI version (AMOE_ABI_VERSION). */
 AMOE_API int amoe_abi_version(void);
 
