@@ -169,6 +169,7 @@ class KVCache:
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._lib = load_library()
+        self._workspace = {}
         self._c = AmoeKvCache(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
                               None if v_scale is None else v_scale.data_ptr(), self.status.data_ptr(), self.pages,
                               self.page_size, self.kv_heads, self.head_dim, kind, k.device.index)
@@ -251,9 +252,19 @@ class KVCache:
             _written(out, "out")
         co = _rows(out, "out", seqs.seqs, self.head_dim, dev)
         attn = _attn(scale, window, sinks, q.shape[1], dev)
+        shape = (seqs.seqs, seqs.table_stride, q.shape[1], window, max_len)
+        size = self._workspace.get(shape)
+        if size is None:  # the library's answer for these shapes
+            size = self._lib.amoe_attn_decode_workspace(ctypes.byref(self._c), ctypes.byref(seqs), q.shape[1], window,
+                                                        max_len)
+            _check(self._lib, min(size, AMOE_OK))
+            if len(self._workspace) > 1000:
+                self._workspace.clear()
+            self._workspace[shape] = size
+        work = _empty((size,), torch.uint8, dev, st) if size else None
         _check(self._lib, self._lib.amoe_attn_decode(
             ctypes.byref(self._c), ctypes.byref(seqs), ctypes.byref(attn), ctypes.byref(cq), ctypes.byref(co),
-            _ints(kv_len, "kv_len", seqs.seqs, dev), max_len, raw))
+            _ints(kv_len, "kv_len", seqs.seqs, dev), max_len, None if work is None else work.data_ptr(), size, raw))
         return out
 
     def check(self):

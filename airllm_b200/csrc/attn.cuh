@@ -124,6 +124,13 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
     return r;
 }
 
+// Four codes of a word, the first two and the last two.
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t four, uint32_t &lo, uint32_t &hi) {
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
+}
+
 // ---- host side ----------------------------------------------------------------------
 inline int reject(const std::string &msg) {
     set_thread_error(msg);
@@ -213,11 +220,14 @@ inline int check_cache(const amoe_kv_cache *c, const amoe_kv_seqs *s) {
         return reject("page_size must be a power of two up to " + std::to_string(kMaxPageSize));
     if (c->kv_heads < 1) return reject("kv_heads must be positive");
     if (c->pages < 1 || c->pages > INT_MAX) return reject("pages outside [1, 2^31)");
+    if (c->pages * c->page_size > (int64_t)UINT32_MAX / c->kv_heads) return reject("cache of 2^32 rows or more");
     if (!c->k || !c->v || !c->status) return reject("cache k, v and status must not be NULL");
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
         return reject("cache k and v must be 16-byte aligned");
     if (c->type == AMOE_KV_E4M3 && (!c->k_scale || !c->v_scale))
         return reject("an E4M3 cache needs k_scale and v_scale");
+    if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15)
+        return reject("cache k_scale and v_scale must be 16-byte aligned");
     if (!s || !s->page_table) return reject("page_table must not be NULL");
     if (s->seqs < 1 || s->table_stride < 1) return reject("seqs and table_stride must be positive");
     return AMOE_OK;

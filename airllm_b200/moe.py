@@ -125,7 +125,8 @@ SIGNATURES = {
     "amoe_kv_append": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "amoe_kv_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "amoe_attn_prefill": (ctypes.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
-    "amoe_attn_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp]),
+    "amoe_attn_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, ctypes.c_int64, _vp]),
+    "amoe_attn_decode_workspace": (ctypes.c_int64, [_vp, _vp, _i32, _i32, _i32]),
 }
 
 GGUF_F32, GGUF_F16, GGUF_BF16, GGUF_MXFP4 = 0, 1, 30, 39

@@ -419,10 +419,17 @@ AMOE_API int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn
  * position kv_len[s] - 1 of sequence s (kv_len [seqs], device, the new token included; 0: a
  * row of zeros).  q and out are F16 or BF16, the cache's type or any with an E4M3 cache.
  * max_len bounds the lengths the call is laid out for (0: the table's capacity); longer
- * ones give the same result in more time. */
+ * ones give the same result in more time.  workspace: amoe_attn_decode_workspace's bytes of
+ * device memory (NULL where that is 0), 16-byte aligned, the call's own until it has run;
+ * its contents before and after mean nothing. */
 AMOE_API int amoe_attn_decode(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const amoe_attn *attn,
                               const amoe_rows *q, const amoe_rows *out, const int32_t *kv_len, int32_t max_len,
-                              void *stream);
+                              void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that amoe_attn_decode needs for these shapes (the cache's and seqs'
+ * device memory is not looked at; no GPU needed), 0 where one launch does; negative: an error. */
+AMOE_API int64_t amoe_attn_decode_workspace(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, int32_t q_heads,
+                                            int32_t window, int32_t max_len);
 
 /* ABI version (AMOE_ABI_VERSION). */
 AMOE_API int amoe_abi_version(void);

@@ -54,7 +54,7 @@ def test_wrong_caches_are_refused(bad, word):
     lib, c, s, r, a = moe.load_library(), cache(**bad), seqs(), rows(), moe.AmoeAttn(0.0, 0, None)
     refused(lib.amoe_kv_append(ref(c), ref(s), AT, AT, 3, None, None, ref(r), ref(r), None, None, None, None), word)
     refused(lib.amoe_kv_read(ref(c), ref(s), AT, None, 3, ref(r), ref(r), None), word)
-    refused(lib.amoe_attn_decode(ref(c), ref(s), ref(a), ref(r), ref(r), AT, 0, None), word)
+    refused(lib.amoe_attn_decode(ref(c), ref(s), ref(a), ref(r), ref(r), AT, 0, None, 0, None), word)
 
 
 @pytest.mark.parametrize("s,word", [(dict(table=None), "page_table"), (dict(stride=0), "positive"), (dict(n=0), "positive")])
@@ -128,7 +128,24 @@ def test_prefill_without_rows_does_nothing():
 def test_decode_refusals(c, q, o, kw, word):
     lib, a = moe.load_library(), moe.AmoeAttn(0.0, 0, None)
     refused(lib.amoe_attn_decode(ref(c), ref(seqs(n=kw.get("n", 2))), ref(a), ref(q), ref(o), kw.get("len", AT),
-                                 kw.get("most", 0), None), word)
+                                 kw.get("most", 0), None, 0, None), word)
+
+
+def test_decode_workspace():
+    lib, a, r = moe.load_library(), moe.AmoeAttn(0.0, 0, None), rows()
+    c = cache(pages=4096, page_size=64)
+    short, long, many = seqs(stride=16, n=1), seqs(stride=2048, n=1), seqs(stride=2048, n=256)
+    def size(s, window=0, most=0):
+        return lib.amoe_attn_decode_workspace(ref(c), ref(s), 8, window, most)
+    # a short context or a large batch needs none, a long one does unless the call bounds it
+    assert size(short) == 0 and size(many) == 0 and size(long) > 0
+    assert size(long, window=128) == 0 and size(long, most=1000) == 0
+    assert lib.amoe_attn_decode_workspace(ref(c), ref(long), 12, 0, 0) == moe.AMOE_ERR_INVALID
+    assert lib.amoe_attn_decode_workspace(ref(c), ref(long), 8, -1, 0) == moe.AMOE_ERR_INVALID
+    assert lib.amoe_attn_decode_workspace(None, ref(long), 8, 0, 0) == moe.AMOE_ERR_INVALID
+    for work, n in ((None, size(long)), (AT, size(long) - 1)):
+        refused(lib.amoe_attn_decode(ref(c), ref(long), ref(a), ref(r), ref(r), AT, 0, work, n, None), "workspace")
+    refused(lib.amoe_attn_decode(ref(c), ref(long), ref(a), ref(r), ref(r), AT, 0, AT + 4, 1 << 40, None), "aligned")
 
 
 @pytest.mark.parametrize("d,theta,yarn", [(64, 150000.0, 1), (128, 150000.0, 1), (64, 10000.0, 0), (2, 500000.0, 1)])

@@ -380,6 +380,20 @@ def test_decode_ignores_what_lies_outside_the_sequence(cuda_device, kind):
     assert torch.isnan(cache.decode(q.cuda(), table.cuda(), i32(lens).cuda(), window=window)).all()
 
 
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_decode_with_far_sinks(cuda_device, kind):
+    g = gen(24)
+    lens = [0, 3, 900]
+    table, pool = table_for(g, lens, 16)
+    pages = filled(g, pool, 2, 16, 64, kind)
+    q = randn(g, 3, 8, 64, dtype=BF16)
+    sinks = torch.tensor([-1e4, 1e4, -300.0, 300.0, 0.0, -math.inf, 60.0, -60.0])
+    got = on_gpu(pages).decode(q.cuda(), table.cuda(), i32(lens).cuda(), sinks=sinks.cuda())
+    assert (got[0] == 0).all()
+    for i in (1, 2):
+        R.close(got[i:i + 1], *R.attention(q[i:i + 1], *(R.rows_of(c, s, table[i], 0, lens[i]) for c, s in pages), sinks))
+
+
 def test_decode_over_scales_far_apart(cuda_device):
     """E4M3 rows whose scales span the whole exponent range, zero rows among them."""
     g = gen(22)
