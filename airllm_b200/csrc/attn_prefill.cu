@@ -1,76 +1,482 @@
 // attn_prefill.cu -- causal attention of packed prompts with grouped heads, learned sinks
-// and a sliding window (CausalAttentionWithConfig, internal/backend/cpuref/attention.go:82-171).
+// and a sliding window (CausalAttentionWithConfig, internal/backend/cpuref/attention.go:82-171),
+// on tcgen05 MMAs with the running maximum and sum of a softmax over key tiles.
 //
 //   s_j = scale q.k_j over the visible keys, m = max s_j,
 //   out = sum exp(s_j - m) v_j / (sum exp(s_j - m) + exp(sink - m))
 //
-// One warp takes one query head's row and walks its keys with a running maximum and sum.
+// One CTA takes 128 rows of one kv head: `group` query heads x 128 / group tokens, so that the
+// keys it stages serve all of them and the diagonal wastes little.  Q, K and V arrive by TMA
+// in 128-byte swizzled rows; S = Q K^T goes to TMEM; four warps (a thread a row) read it back, keep the
+// row's maximum and sum, and write the weights, rounded to the inputs' type, to TMEM, where they are
+// the A operand of O += P V.  V is staged as it lies in memory ([keys][d], the MN-major B operand).  S is read into
+// registers at once, so the next tile's Q K^T runs under this tile's exponentials; and two CTAs share an
+// SM (256 TMEM columns each), so one's products run under the other's softmax.
+//
+// The maximum is lazy: O and the sum are rescaled only when a row's maximum has grown by more
+// than 2^8 since the last time, which float32 sums and 16-bit weights (relative precision) hold without loss.
+//
+// A key that a row must not see has weight 0, but 0 times an infinity or NaN in its value is NaN.
+// Values behind the tile's last visible key are overwritten with zeros in shared memory; a row whose
+// result is still not finite is computed again by its thread, key by visible key.  Finite inputs never take that path.
 #include "attn.cuh"
+#include "tc_ptx.cuh"
+
+#include <atomic>
 
 namespace amoe {
 namespace attn {
 namespace {
 
-constexpr int kThreads = 128;
+using bs::mbar_arrive;
+using bs::mbar_expect_tx;
+using bs::mbar_init;
+using bs::smem_u32;
+using bs::tc_fence_after;
+using bs::tc_fence_before;
+
+constexpr int kRows = 128;
+constexpr int kSoftWarps = 4, kMmaWarp = 4, kTmaWarp = 5;
+constexpr int kThreads = 192;
+constexpr int kStages = 2;
+constexpr int kTmemCols = 256;
+constexpr float kLazy = 8.0f;  // log2 growth of a row's maximum that is left in the weights
 
 struct PrefillParams {
-    RowsDev q, k, v, out;
+    RowsDev q, k, v, out;  // K and V for the rows that are computed again
     const int32_t *cu_q, *cu_k;
     const float *sinks;
     float scale_log2;
-    int window, q_tokens, k_tokens, seqs, q_heads, group;
+    int window, q_tokens, k_tokens, seqs, group, tile_tokens;
 };
 
-template <int D, int TYPE>
-__global__ void __launch_bounds__(kThreads) prefill_kernel(const __grid_constant__ PrefillParams p) {
-    constexpr int E = D / 32;  // elements of a lane
+template <int D>
+struct Cfg {
+    static constexpr int N = D == 64 ? 128 : 64;  // keys of a tile
+    static constexpr int kHalves = D / 64;        // 128-byte column blocks of a row
+    static constexpr int kQBytes = kRows * D * 2;
+    static constexpr int kTileBytes = N * D * 2;
+    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + 256;
+    static constexpr int kS = 0, kP = N, kO = N + N / 2;  // TMEM columns
+    static_assert(kO + D <= kTmemCols, "TMEM columns");
+};
+
+// What a CTA works on, found by one warp and shared.
+struct Work {
+    int tok0, tokens;    // first query row and how many of the tile's are the sequence's
+    int at0;             // position of the first among its keys
+    int k0, lo, hi;      // the sequence's first key row; visible keys [lo, hi) of the tile
+    int dead;            // a bounded wait gave up
+    int found;
+};
+
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, Work *w) {
+    return bs::mbar_wait(bar, parity, &w->dead, 1);
+}
+
+// The same for a whole warp, which stays together when a wait gives up.
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, Work *w) {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, w));
+}
+
+__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *tm, uint64_t *bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Operand in 128-byte swizzled rows, eight-row groups 1024 bytes apart.  lbo: bytes between 64-column
+// blocks, which only the MN-major operand of 128 columns has.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+           (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+
+// kind::f16: f32 accumulators, both operands of TYPE, M = 128.
+template <int TYPE>
+__device__ __forceinline__ uint32_t idesc(int n, bool b_mn) {
+    const uint32_t t = TYPE == AMOE_GGUF_F16 ? 0u : 1u;
+    return 1u << 4 | t << 7 | t << 10 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(id), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+
+// 16 columns of this warp's lanes.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One warp finds the sequence and tile of CTA x: sequences in order, each one's last (longest) tile first.
+__device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w) {
     const int lane = threadIdx.x % 32;
-    const int t = blockIdx.x, h = blockIdx.y * (kThreads / 32) + threadIdx.x / 32;
-    if (h >= p.q_heads) return;
-    if (t >= p.cu_q[p.seqs]) return;
-    const int s = find_seq(p.cu_q, p.seqs, t);
-    const int q0 = p.cu_q[s], q1 = min(p.cu_q[s + 1], p.q_tokens);
-    if (q0 < 0 || t < q0 || t >= q1) return;
-    const int k0 = max(p.cu_k[s], 0), k1 = min(p.cu_k[s + 1], p.k_tokens);
-    const int at = (k1 - k0) - (q1 - t);  // this query's position among its keys
-    const int from = p.window > 0 ? max(0, at - p.window + 1) : 0;
-    auto row = [&](const RowsDev &r, int tok, int head, float (&x)[E]) {
-        const char *src = r.p + tok * r.ts + head * r.hs + lane * E * 2;
+    int before = 0;
+    for (int s0 = 0; s0 < p.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int a = 0, b = 0, tiles = 0;
+        if (s < p.seqs) {
+            a = p.cu_q[s], b = min(p.cu_q[s + 1], p.q_tokens);
+            if (a >= 0 && a < b) tiles = (b - a - 1) / p.tile_tokens + 1;
+        }
+        int upto = tiles;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            x[i] = TYPE == AMOE_GGUF_F16 ? __half2float(reinterpret_cast<const __half *>(src)[i])
-                                         : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(src)[i]);
-    };
-    float q[E], acc[E] = {}, m = -INFINITY, l = 0.0f;
-    row(p.q, t, h, q);
+        for (int i = 1; i < 32; i <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, i);
+            if (lane >= i) upto += y;
+        }
+        const bool mine = tiles > 0 && x >= before + upto - tiles && x < before + upto;
+        if (mine) {
+            const int tile = before + upto - 1 - x;  // the last one first
+            const int k0 = max(p.cu_k[s], 0), k1 = min(p.cu_k[s + 1], p.k_tokens);
+            const int klen = max(k1 - k0, 0);
+            w->tok0 = a + tile * p.tile_tokens;
+            w->tokens = min(p.tile_tokens, b - w->tok0);
+            w->at0 = klen - (b - w->tok0);
+            w->k0 = k0;
+            w->hi = max(w->at0 + w->tokens, 0);
+            w->lo = p.window > 0 ? max(w->at0 - p.window + 1, 0) : 0;
+            w->dead = 0;
+        }
+        if (__any_sync(0xffffffffu, mine)) return true;
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+// A row again, key by visible key: for results that are not finite.
+template <int D, int TYPE>
+__device__ __noinline__ void row_again(const PrefillParams &p, int tok, int head, int k0, int from, int at) {
+    float acc[D], q[D], m = -INFINITY, l = 0.0f;
+    const int kvh = head / p.group;
+    for (int d = 0; d < D; d += 8) {
+        load8<TYPE>(p.q.p + tok * p.q.ts + head * p.q.hs + d * 2, *reinterpret_cast<float(*)[8]>(q + d));
+        for (int i = 0; i < 8; ++i) acc[d + i] = 0.0f;
+    }
     for (int j = from; j <= at; ++j) {
-        float k[E], v[E], dot = 0.0f;
-        row(p.k, k0 + j, h / p.group, k);
-        row(p.v, k0 + j, h / p.group, v);
-#pragma unroll
-        for (int i = 0; i < E; ++i) dot = fmaf(q[i], k[i], dot);
-#pragma unroll
-        for (int w = 16; w; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-        const float x = dot * p.scale_log2, mm = fmaxf(m, x);
-        const float keep = mm == -INFINITY ? 1.0f : exp2f(m - mm), e = mm == -INFINITY ? 0.0f : exp2f(x - mm);
+        const char *k = p.k.p + (k0 + j) * p.k.ts + kvh * p.k.hs, *v = p.v.p + (k0 + j) * p.v.ts + kvh * p.v.hs;
+        float x[8], dot = 0.0f;
+        for (int d = 0; d < D; d += 8) {
+            load8<TYPE>(k + d * 2, x);
+            for (int i = 0; i < 8; ++i) dot = fmaf(q[d + i], x[i], dot);
+        }
+        const float s = dot * p.scale_log2, mm = fmaxf(m, s), z = mm == -INFINITY ? 0.0f : mm;
+        const float keep = exp2f(m - z), e = exp2f(s - z);
         m = mm;
         l = l * keep + e;
-#pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] = acc[i] * keep + e * v[i];
+        for (int d = 0; d < D; d += 8) {
+            load8<TYPE>(v + d * 2, x);
+            for (int i = 0; i < 8; ++i) acc[d + i] = acc[d + i] * keep + e * x[i];
+        }
     }
-    if (p.sinks) {
-        const float x = p.sinks[h] * kLog2e, mm = fmaxf(m, x);
-        const float keep = mm == -INFINITY ? 1.0f : exp2f(m - mm);
-        l = l * keep + (mm == -INFINITY ? 0.0f : exp2f(x - mm));
-#pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] *= keep;
+    const float z = m == -INFINITY ? 0.0f : m;
+    if (p.sinks) l += exp2f(p.sinks[head] * kLog2e - z);
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int d = 0; d < D; d += 8) {
+        float x[8];
+        for (int i = 0; i < 8; ++i) x[i] = acc[d + i] * by;
+        store8<TYPE>(p.out.p + tok * p.out.ts + head * p.out.hs + d * 2, x);
     }
-    char *dst = p.out.p + t * p.out.ts + h * p.out.hs + lane * E * 2;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-        const float r = l == 0.0f ? 0.0f : 1.0f / l;
-        reinterpret_cast<uint32_t *>(dst)[i / 2] = pack2<TYPE>(acc[i] * r, acc[i + 1] * r);
+}
+
+template <int D, int TYPE>
+__global__ void __launch_bounds__(kThreads, 2)
+    prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
+    using C = Cfg<D>;
+    constexpr int N = C::N, HALVES = C::kHalves;
+    extern __shared__ __align__(1024) uint8_t sm_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *q_s = sm, *k_s = q_s + C::kQBytes, *v_s = k_s + kStages * C::kTileBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(v_s + kStages * C::kTileBytes);
+    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages;
+    uint64_t *v_empty = v_full + kStages, *s_full = v_empty + kStages, *s_free = s_full + 1, *p_full = s_free + 1;
+    uint64_t *o_done = p_full + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_done + 1);
+    Work *work = reinterpret_cast<Work *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int kvh = blockIdx.y;
+    if (warp == 0) {
+        const bool f = find_work(p, blockIdx.x, work);
+        if (lane == 0) work->found = f;
     }
+    if (threadIdx.x == 32) {
+        mbar_init(q_full, 1);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1);
+            mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+        }
+        mbar_init(s_full, 1), mbar_init(o_done, 1);
+        mbar_init(s_free, kSoftWarps), mbar_init(p_full, kSoftWarps);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (!work->found) return;
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "n"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int tok0 = work->tok0, at0 = work->at0, lo = work->lo, hi = work->hi, k0 = work->k0;
+    const int tiles = hi > lo ? (hi - lo - 1) / N + 1 : 0;
+    // columns of the last tile that hold a visible key, in whole MMA steps
+    const int last_cols = tiles > 0 ? (hi - lo - (tiles - 1) * N + 15) / 16 * 16 : 0;
+
+    if (warp == kTmaWarp) {
+        if (lane == 0 && tiles > 0) {
+            mbar_expect_tx(q_full, p.tile_tokens * p.group * D * 2);
+            for (int h = 0; h < HALVES; ++h) tma_3d(q_s + h * kRows * 128, &tm_q, q_full, h * 64, kvh * p.group, tok0);
+            for (int j = 0; j < tiles; ++j) {
+                const int s = j % kStages, row = k0 + lo + j * N;
+                const uint32_t ph = (uint32_t)(j / kStages - 1) & 1u;
+                if (j >= kStages && !wait_bar(k_empty + s, ph, work)) break;
+                mbar_expect_tx(k_full + s, C::kTileBytes);
+                for (int h = 0; h < HALVES; ++h)
+                    tma_3d(k_s + s * C::kTileBytes + h * N * 128, &tm_k, k_full + s, h * 64, kvh, row);
+                if (j >= kStages && !wait_bar(v_empty + s, ph, work)) break;
+                mbar_expect_tx(v_full + s, C::kTileBytes);
+                for (int h = 0; h < HALVES; ++h)
+                    tma_3d(v_s + s * C::kTileBytes + h * N * 128, &tm_v, v_full + s, h * 64, kvh, row);
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        const uint32_t q_a = smem_u32(q_s), k_a = smem_u32(k_s), v_a = smem_u32(v_s);
+        bool ok = tiles > 0 && wait_warp(q_full, 0, work);
+        for (int j = 0; ok && j <= tiles; ++j) {
+            if (j < tiles) {  // S = Q K^T of tile j
+                const int s = j % kStages;
+                ok = wait_warp(k_full + s, (uint32_t)(j / kStages) & 1u, work);
+                if (ok && j > 0) ok = wait_warp(s_free, (uint32_t)(j - 1) & 1u, work);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t id = idesc<TYPE>(j + 1 == tiles ? last_cols : N, false);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t off = i / 4, in = i % 4 * 32;
+                        mma_ss(tmem + C::kS, desc_sw128(q_a + off * kRows * 128 + in, 16),
+                               desc_sw128(k_a + s * C::kTileBytes + off * N * 128 + in, 16), id, i > 0);
+                    }
+                    mma_commit(s_full);
+                    mma_commit(k_empty + s);
+                }
+                __syncwarp();
+            }
+            if (j > 0) {  // O += P V of tile j - 1
+                const int t = j - 1, s = t % kStages;
+                ok = wait_warp(v_full + s, (uint32_t)(t / kStages) & 1u, work);
+                if (!ok) break;
+                const int cols = t + 1 == tiles ? last_cols : N;
+                const int seen = hi - lo - t * N;
+                if (seen < cols) {  // no value behind the last visible key reaches the products
+                    for (int i = lane; i < (cols - seen) * 8 * HALVES; i += 32) {
+                        const int h = i / ((cols - seen) * 8), r = i / 8 % (cols - seen);
+                        *reinterpret_cast<uint4 *>(v_s + s * C::kTileBytes + h * N * 128 + (seen + r) * 128 + i % 8 * 16) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                ok = wait_warp(p_full, (uint32_t)t & 1u, work);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t id = idesc<TYPE>(D, true);
+                    for (int i = 0; i < cols / 16; ++i)
+                        mma_ts(tmem + C::kO, tmem + C::kP + i * 8,
+                               desc_sw128(v_a + s * C::kTileBytes + i * 2048, N * 128), id, t > 0 || i > 0);
+                    mma_commit(o_done);
+                    mma_commit(v_empty + s);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // a thread's row: token r / group of the tile, query head r % group of the kv head
+        const int r = threadIdx.x, tok = r / p.group, head = kvh * p.group + r % p.group;
+        const int at = at0 + tok;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            ok = wait_warp(s_full, (uint32_t)j & 1u, work);
+            if (!ok) break;
+            tc_fence_after();
+            const int base = lo + j * N, cols = j + 1 == tiles ? last_cols : N;
+            float s[N];
+#pragma unroll
+            for (int c = 0; c < N; c += 32) {
+                if (c < cols) {
+                    bs::tmem_ld32(tmem + lanes + C::kS + c, *reinterpret_cast<float(*)[32]>(s + c));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c + i] = -INFINITY;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free);
+            if (base + N - 1 > at0 || (p.window > 0 && base <= hi - 1 - p.window)) {
+                const int last = at - base, first = p.window > 0 ? at - p.window + 1 - base : 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (i > last || i < first) s[i] = -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < N; ++i) top = fmaxf(top, s[i]);
+            const bool grown = (top - m) * p.scale_log2 > kLazy;
+            bool waited = j == 0;
+            if (__any_sync(0xffffffffu, grown)) {
+                const float mm = fmaxf(m, top);
+                if (j > 0) {
+                    ok = wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
+                    if (!ok) break;
+                    waited = true;
+                    tc_fence_after();
+                    const float keep = mm == -INFINITY ? 1.0f : ex2((m - mm) * p.scale_log2);
+                    l *= keep;
+#pragma unroll
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        bs::tmem_ld16(tmem + lanes + C::kO + c, o);
+                        uint32_t u[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * keep);
+                        tmem_st16(tmem + lanes + C::kO + c, u);
+                    }
+                }
+                m = mm;
+            }
+            const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < N; c += 32) {
+                if (c >= cols) break;
+                uint32_t u[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float a = ex2(fmaf(s[c + 2 * i], p.scale_log2, -off));
+                    const float b = ex2(fmaf(s[c + 2 * i + 1], p.scale_log2, -off));
+                    sum += a + b;
+                    u[i] = pack2<TYPE>(a, b);
+                }
+                if (!waited) {  // the products of the tile before have read P
+                    ok = wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
+                    waited = true;
+                    tc_fence_after();
+                }
+                tmem_st16(tmem + lanes + C::kP + c / 2, u);
+            }
+            if (!ok) break;
+            l += sum;
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full);
+        }
+        if (ok && tiles > 0) ok = wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
+        tc_fence_after();
+        const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
+        const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
+        if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - off);
+        const float by = !ok ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
+        bool fine = true;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+            float o[32];
+            __syncwarp();
+            if (tiles > 0) {
+                bs::tmem_ld32(tmem + lanes + C::kO + c, o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+            }
+            float worst = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;  // 0, or NaN
+            fine &= worst == 0.0f;
+            if (mine) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = o[i + e] * by;
+                    store8<TYPE>(dst + (c + i) * 2, x);
+                }
+            }
+        }
+        if (mine && ok && (!fine || !isfinite(l)))
+            row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols));
+    }
+}
+
+// [tokens][heads][D] rows as a 3-D map with boxes of 64 elements x heads x tokens.
+bool encode_rows(CUtensorMap *tm, const amoe_rows *r, int D, int tokens, int box_heads, int box_tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)r->heads, (cuuint64_t)(tokens > 0 ? tokens : 1)};
+    // the stride of a dimension of one is never used, but has to be a valid one
+    const cuuint64_t strides[2] = {(cuuint64_t)(r->heads > 1 ? r->head_stride * 2 : D * 2),
+                                   (cuuint64_t)(tokens > 1 ? r->token_stride * 2 : D * 2)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, es[3] = {1, 1, 1};
+    return bs::encode_fn()(tm, r->type == AMOE_GGUF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                           3, r->data, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kMaxDevices = 64;
+
+template <int D, int TYPE>
+cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PrefillParams &p, int device,
+                   dim3 grid, cudaStream_t st) {
+    auto *kernel = prefill_kernel<D, TYPE>;
+    static std::atomic<bool> ready[kMaxDevices];
+    if (!ready[device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+        if (e != cudaSuccess) return e;
+        ready[device].store(true, std::memory_order_release);
+    }
+    kernel<<<grid, kThreads, Cfg<D>::kSmem, st>>>(q, k, v, p);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -95,6 +501,8 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     if (int rc = check_group(q->heads, k->heads)) return rc;
     if (!cu_q || !cu_k) return reject("cu_q and cu_k must not be NULL");
     if (seqs < 1) return reject("seqs must be positive");
+    if (k->heads > 65535) return reject("more than 65535 kv heads in one prefill call");
+    if (device < 0 || device >= kMaxDevices) return reject("device ordinal out of range");
     if (q_tokens == 0) return AMOE_OK;
     PrefillParams p{};
     p.q = rows_dev(q), p.k = rows_dev(k), p.v = rows_dev(v), p.out = rows_dev(out);
@@ -102,16 +510,30 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     p.sinks = attn->sinks;
     p.scale_log2 = attn_scale(attn, head_dim) * kLog2e;
     p.window = attn->window, p.q_tokens = q_tokens, p.k_tokens = k_tokens, p.seqs = seqs;
-    p.q_heads = q->heads, p.group = q->heads / k->heads;
+    p.group = q->heads / k->heads;
+    p.tile_tokens = kRows / p.group;
+    // every sequence's last tile may be a short one
+    const int64_t tiles = (int64_t)q_tokens / p.tile_tokens + (seqs < q_tokens ? seqs : q_tokens);
+    if (tiles > INT_MAX) return reject("too many query rows");
     DeviceScope scope;
     cudaError_t e = scope.enter(device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
+    if (!bs::get_encode()) {
+        set_thread_error("cuTensorMapEncodeTiled is not available");
+        return AMOE_ERR_CUDA;
+    }
+    const int n = head_dim == 64 ? Cfg<64>::N : Cfg<128>::N;
+    CUtensorMap tq, tk, tv;
+    if (!encode_rows(&tq, q, head_dim, q_tokens, p.group, p.tile_tokens) ||
+        !encode_rows(&tk, k, head_dim, k_tokens, 1, n) || !encode_rows(&tv, v, head_dim, k_tokens, 1, n))
+        return reject("prefill: strides of q, k or v that a tensor map cannot take");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid(q_tokens, (q->heads + 3) / 4);
-    if (head_dim == 64 && q->type == AMOE_GGUF_F16) prefill_kernel<64, AMOE_GGUF_F16><<<grid, kThreads, 0, st>>>(p);
-    else if (head_dim == 64) prefill_kernel<64, AMOE_GGUF_BF16><<<grid, kThreads, 0, st>>>(p);
-    else if (q->type == AMOE_GGUF_F16) prefill_kernel<128, AMOE_GGUF_F16><<<grid, kThreads, 0, st>>>(p);
-    else prefill_kernel<128, AMOE_GGUF_BF16><<<grid, kThreads, 0, st>>>(p);
-    e = cudaGetLastError();
+    const dim3 grid((unsigned)tiles, k->heads);
+    if (head_dim == 64)
+        e = q->type == AMOE_GGUF_F16 ? launch<64, AMOE_GGUF_F16>(tq, tk, tv, p, device, grid, st)
+                                     : launch<64, AMOE_GGUF_BF16>(tq, tk, tv, p, device, grid, st);
+    else
+        e = q->type == AMOE_GGUF_F16 ? launch<128, AMOE_GGUF_F16>(tq, tk, tv, p, device, grid, st)
+                                     : launch<128, AMOE_GGUF_BF16>(tq, tk, tv, p, device, grid, st);
     return e == cudaSuccess ? AMOE_OK : cuda_error(e, "prefill kernel");
 }
