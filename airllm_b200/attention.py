@@ -26,11 +26,12 @@ skipped there and reported by ``KVCache.check``.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from .moe import (AMOE_ERR_INVALID, AMOE_OK, GGUF_BF16, GGUF_F16, GGUF_F32, KV_BAD_LENGTHS, KV_BAD_PAGE, KV_E4M3,
-                  KV_PAST_TABLE, AmoeAttn, AmoeError, AmoeKvCache, AmoeKvSeqs, AmoeRope, AmoeRows, load_library)
+                  KV_PAST_TABLE, AmoeError, AmoeKvCache, AmoeRope, load_library)
 
 _TYPES = {torch.float32: GGUF_F32, torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16}
 _CACHE_TYPES = {torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16, torch.float8_e4m3fn: KV_E4M3}
@@ -45,12 +46,20 @@ def _check(lib, rc: int):
         raise AmoeError(rc, lib.amoe_last_error(None).decode())
 
 
-def _rows(t, name: str, tokens: int, head_dim: int, device) -> AmoeRows:
+# The C structures of include/amoe.h, packed: a bytes object is a pointer to ctypes, and packing
+# one costs a fraction of building a ctypes.Structure.
+_pack_rows = struct.Struct("Pqqii").pack  # amoe_rows
+_pack_seqs = struct.Struct("Pii").pack    # amoe_kv_seqs
+_pack_attn = struct.Struct("fiP").pack    # amoe_attn
+
+
+def _rows(t, name: str, tokens: int, head_dim: int, device: int) -> bytes:
     """A [tokens, heads, head_dim] tensor as the C ABI's rows."""
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != head_dim:
-        _invalid(f"{name} must be [{tokens}, heads, {head_dim}], got {list(t.shape)}")
-    if t.device != device:
-        _invalid(f"{name} is on {t.device}, want {device}")
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
+        _invalid(f"{name} must be [{tokens}, heads, {head_dim}], got {list(shape)}")
+    if t.get_device() != device:
+        _invalid(f"{name} is on {t.device}, want cuda:{device}")
     kind = _TYPES.get(t.dtype)
     if kind is None:
         _invalid(f"{name} has type {t.dtype}")
@@ -58,7 +67,7 @@ def _rows(t, name: str, tokens: int, head_dim: int, device) -> AmoeRows:
     if sd != 1:
         _invalid(f"{name}: the elements of a row must be adjacent")
     # a call without rows has no address to give
-    return AmoeRows(t.data_ptr() or 16, st, sh, t.shape[1], kind)
+    return _pack_rows(t.data_ptr() or 16, st, sh, shape[1], kind)
 
 
 def _written(t, name: str):
@@ -70,22 +79,22 @@ def _written(t, name: str):
         _invalid(f"{name}: its rows overlap")
 
 
-def _ints(t, name: str, n: int, device) -> int:
+def _ints(t, name: str, n: int, device: int) -> int:
     if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         _invalid(f"{name} must be {n} adjacent int32 values")
-    if t.device != device:
-        _invalid(f"{name} is on {t.device}, want {device}")
+    if t.get_device() != device:
+        _invalid(f"{name} is on {t.device}, want cuda:{device}")
     return t.data_ptr()
 
 
-def _stream(stream, device):
+def _stream(stream, device: int):
     """(the raw stream, a torch stream to allocate under or None for the current one)."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, None
+        return torch._C._cuda_getCurrentRawStream(device), None
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
-    if stream.device != device:
-        _invalid(f"stream is on {stream.device}, want {device}")
+    if stream.device.index != device:
+        _invalid(f"stream is on {stream.device}, want cuda:{device}")
     return stream.cuda_stream, stream
 
 
@@ -96,17 +105,21 @@ def _empty(shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _attn(scale, window: int, sinks, heads: int, device) -> AmoeAttn:
-    if scale is not None and not scale > 0:
+def _attn(scale, window: int, sinks, heads: int, device: int) -> bytes:
+    if scale is None:
+        scale = 0.0
+    elif not scale > 0:
         _invalid("scale must be positive")
-    at = None
+    at = 0
     if sinks is not None:
         if sinks.dtype != torch.float32 or sinks.dim() != 1 or sinks.shape[0] != heads or not sinks.is_contiguous():
             _invalid(f"sinks must be {heads} adjacent float32 values")
-        if sinks.device != device:
-            _invalid(f"sinks is on {sinks.device}, want {device}")
+        if sinks.get_device() != device:
+            _invalid(f"sinks is on {sinks.device}, want cuda:{device}")
         at = sinks.data_ptr()
-    return AmoeAttn(scale or 0.0, window, at)
+    if not -(1 << 31) <= window < 1 << 31:
+        _invalid("window must fit 32 bits")
+    return _pack_attn(scale, window, at)
 
 
 class Rope:
@@ -115,7 +128,8 @@ class Rope:
     def __init__(self, head_dim: int, theta: float = 150000.0, yarn: bool = True):
         lib = load_library()
         self._c = AmoeRope()
-        _check(lib, lib.amoe_rope_init(head_dim, theta, 1 if yarn else 0, ctypes.byref(self._c)))
+        self._at = ctypes.addressof(self._c)
+        _check(lib, lib.amoe_rope_init(head_dim, theta, 1 if yarn else 0, self._at))
 
     @property
     def frequencies(self) -> list:
@@ -173,14 +187,17 @@ class KVCache:
         self._c = AmoeKvCache(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
                               None if v_scale is None else v_scale.data_ptr(), self.status.data_ptr(), self.pages,
                               self.page_size, self.kv_heads, self.head_dim, kind, k.device.index)
+        self._at, self._index = ctypes.addressof(self._c), k.device.index
 
-    def _seqs(self, page_table) -> AmoeKvSeqs:
+    def _seqs(self, page_table):
+        """(the C ABI's sequences, how many)."""
         t = page_table
-        if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.device != self.device:
-            _invalid(f"page_table must be int32 [seqs, pages] with adjacent columns on {self.device}")
-        if t.shape[0] < 1 or t.shape[1] < 1 or (t.shape[0] > 1 and t.stride(0) != t.shape[1]):
-            _invalid("page_table must be contiguous and not empty")
-        return AmoeKvSeqs(t.data_ptr(), t.shape[1], t.shape[0])
+        shape = t.shape
+        if t.dtype != torch.int32 or len(shape) != 2 or not t.is_contiguous() or min(shape) < 1:
+            _invalid("page_table must be int32 [seqs, pages], contiguous and not empty")
+        if t.get_device() != self._index:
+            _invalid(f"page_table is on {t.device}, want {self.device}")
+        return _pack_seqs(t.data_ptr(), shape[1], shape[0]), shape[0]
 
     def append(self, k, v, page_table, past, cu, q=None, rope: Rope | None = None, q_type=None, q_out=None,
                k_out=None, v_out=None, stream=None):
@@ -188,83 +205,88 @@ class KVCache:
         [tokens, kv_heads, head_dim] become sequence s's tokens past[s], past[s] + 1, ...
         Returns the rotated q [tokens, q_heads, head_dim] (``q_out``, or a new tensor of
         ``q_type``, by default q's own), None without q."""
-        n, dev = k.shape[0], self.device
-        seqs = self._seqs(page_table)
+        n, d, dev = k.shape[0], self.head_dim, self._index
+        seqs, count = self._seqs(page_table)
         raw, st = _stream(stream, dev)
-        ck, cv = _rows(k, "k", n, self.head_dim, dev), _rows(v, "v", n, self.head_dim, dev)
         cq = cqo = cko = cvo = None
         if q is not None:
-            cq = _rows(q, "q", n, self.head_dim, dev)
+            cq = _rows(q, "q", n, d, dev)
             if q_out is None:
-                q_out = _empty(q.shape, q_type or q.dtype, dev, st)
-            elif q_type is not None and q_out.dtype != q_type:
-                _invalid(f"q_out is {q_out.dtype}, q_type {q_type}")
+                q_out = _empty(q.shape, q_type or q.dtype, self.device, st)
+            else:
+                if q_type is not None and q_out.dtype != q_type:
+                    _invalid(f"q_out is {q_out.dtype}, q_type {q_type}")
+                _written(q_out, "q_out")
+            cqo = _rows(q_out, "q_out", n, d, dev)
         elif q_out is not None:
             _invalid("q_out without q")
-        if q_out is not None:
-            _written(q_out, "q_out")
-            cqo = ctypes.byref(_rows(q_out, "q_out", n, self.head_dim, dev))
         if k_out is not None:
             _written(k_out, "k_out")
-            cko = ctypes.byref(_rows(k_out, "k_out", n, self.head_dim, dev))
+            cko = _rows(k_out, "k_out", n, d, dev)
         if v_out is not None:
             _written(v_out, "v_out")
-            cvo = ctypes.byref(_rows(v_out, "v_out", n, self.head_dim, dev))
-        _check(self._lib, self._lib.amoe_kv_append(
-            ctypes.byref(self._c), ctypes.byref(seqs), _ints(cu, "cu", seqs.seqs + 1, dev),
-            _ints(past, "past", seqs.seqs, dev), n, None if rope is None else ctypes.byref(rope._c),
-            None if cq is None else ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv), cqo, cko, cvo, raw))
+            cvo = _rows(v_out, "v_out", n, d, dev)
+        rc = self._lib.amoe_kv_append(
+            self._at, seqs, _ints(cu, "cu", count + 1, dev), _ints(past, "past", count, dev), n,
+            None if rope is None else rope._at, cq, _rows(k, "k", n, d, dev), _rows(v, "v", n, d, dev), cqo, cko, cvo,
+            raw)
+        if rc:
+            _check(self._lib, rc)
         return q_out
 
     def read(self, page_table, cu, total: int, dtype=None, first=None, k_out=None, v_out=None, stream=None):
         """Sequence s's keys and values from position first[s] (default 0) on as packed rows
         cu[s]..cu[s+1] (amoe_kv_read).  Returns (k, v) [total, kv_heads, head_dim]: k_out and v_out,
         or new tensors of ``dtype`` (default: the cache's own type, bfloat16 for E4M3)."""
-        dev = self.device
-        seqs = self._seqs(page_table)
+        d, dev = self.head_dim, self._index
+        seqs, count = self._seqs(page_table)
         raw, st = _stream(stream, dev)
         if dtype is None:
-            dtype = torch.bfloat16 if self._c.type == KV_E4M3 else self.k.dtype
-        shape = (total, self.kv_heads, self.head_dim)
-        k_out = _empty(shape, dtype, dev, st) if k_out is None else k_out
-        v_out = _empty(shape, dtype, dev, st) if v_out is None else v_out
-        _written(k_out, "k_out")
-        _written(v_out, "v_out")
-        ck = _rows(k_out, "k_out", total, self.head_dim, dev)
-        cv = _rows(v_out, "v_out", total, self.head_dim, dev)
-        _check(self._lib, self._lib.amoe_kv_read(
-            ctypes.byref(self._c), ctypes.byref(seqs), _ints(cu, "cu", seqs.seqs + 1, dev),
-            None if first is None else _ints(first, "first", seqs.seqs, dev), total, ctypes.byref(ck),
-            ctypes.byref(cv), raw))
+            dtype = torch.bfloat16 if self.k_scale is not None else self.k.dtype
+        shape = (total, self.kv_heads, d)
+        if k_out is None:
+            k_out = _empty(shape, dtype, self.device, st)
+        else:
+            _written(k_out, "k_out")
+        if v_out is None:
+            v_out = _empty(shape, dtype, self.device, st)
+        else:
+            _written(v_out, "v_out")
+        rc = self._lib.amoe_kv_read(
+            self._at, seqs, _ints(cu, "cu", count + 1, dev),
+            None if first is None else _ints(first, "first", count, dev), total, _rows(k_out, "k_out", total, d, dev),
+            _rows(v_out, "v_out", total, d, dev), raw)
+        if rc:
+            _check(self._lib, rc)
         return k_out, v_out
 
     def decode(self, q, page_table, kv_len, scale: float | None = None, window: int = 0, sinks=None,
                max_len: int = 0, out=None, stream=None):
         """Attention of one new token a sequence (amoe_attn_decode): q [seqs, q_heads, head_dim] at
         position kv_len[s] - 1.  Returns out, like q."""
-        dev = self.device
-        seqs = self._seqs(page_table)
+        d, dev = self.head_dim, self._index
+        seqs, count = self._seqs(page_table)
         raw, st = _stream(stream, dev)
-        cq = _rows(q, "q", seqs.seqs, self.head_dim, dev)
+        cq = _rows(q, "q", count, d, dev)
+        heads = q.shape[1]
         if out is None:
-            out = _empty(q.shape, q.dtype, dev, st)
+            out = _empty((count, heads, d), q.dtype, self.device, st)
         else:
             _written(out, "out")
-        co = _rows(out, "out", seqs.seqs, self.head_dim, dev)
-        attn = _attn(scale, window, sinks, q.shape[1], dev)
-        shape = (seqs.seqs, seqs.table_stride, q.shape[1], window, max_len)
+        shape = (count, page_table.shape[1], heads, window, max_len)
         size = self._workspace.get(shape)
         if size is None:  # the library's answer for these shapes
-            size = self._lib.amoe_attn_decode_workspace(ctypes.byref(self._c), ctypes.byref(seqs), q.shape[1], window,
-                                                        max_len)
+            size = self._lib.amoe_attn_decode_workspace(self._at, seqs, heads, window, max_len)
             _check(self._lib, min(size, AMOE_OK))
             if len(self._workspace) > 1000:
                 self._workspace.clear()
             self._workspace[shape] = size
-        work = _empty((size,), torch.uint8, dev, st) if size else None
-        _check(self._lib, self._lib.amoe_attn_decode(
-            ctypes.byref(self._c), ctypes.byref(seqs), ctypes.byref(attn), ctypes.byref(cq), ctypes.byref(co),
-            _ints(kv_len, "kv_len", seqs.seqs, dev), max_len, None if work is None else work.data_ptr(), size, raw))
+        work = _empty((size,), torch.uint8, self.device, st) if size else None
+        rc = self._lib.amoe_attn_decode(
+            self._at, seqs, _attn(scale, window, sinks, heads, dev), cq, _rows(out, "out", count, d, dev),
+            _ints(kv_len, "kv_len", count, dev), max_len, None if work is None else work.data_ptr(), size, raw)
+        if rc:
+            _check(self._lib, rc)
         return out
 
     def check(self):
@@ -285,21 +307,23 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: float | None = None, window: int = 
     [tokens, q_heads, head_dim] are the last of the positions that rows cu_k[s]..cu_k[s+1] of
     k and v [keys, kv_heads, head_dim] hold (cu_k None: cu_q).  Returns out, like q."""
     lib = load_library()
-    dev = q.device
-    if not q.is_cuda or q.dim() != 3:
+    dev = q.get_device()
+    if dev < 0 or q.dim() != 3:
         _invalid("q must be a CUDA tensor [tokens, q_heads, head_dim]")
-    cu_k = cu_q if cu_k is None else cu_k
+    if cu_k is None:
+        cu_k = cu_q
     seqs = cu_q.shape[0] - 1
     raw, st = _stream(stream, dev)
-    n, m, d = q.shape[0], k.shape[0], q.shape[2]
+    n, heads, d = q.shape
+    m = k.shape[0]
     if out is None:
-        out = _empty(q.shape, q.dtype, dev, st)
+        out = _empty((n, heads, d), q.dtype, q.device, st)
     else:
         _written(out, "out")
-    cq, co = _rows(q, "q", n, d, dev), _rows(out, "out", n, d, dev)
-    ck, cv = _rows(k, "k", m, d, dev), _rows(v, "v", m, d, dev)
-    attn = _attn(scale, window, sinks, q.shape[1], dev)
-    _check(lib, lib.amoe_attn_prefill(
-        dev.index, d, ctypes.byref(attn), ctypes.byref(cq), ctypes.byref(ck), ctypes.byref(cv), ctypes.byref(co),
-        n, m, _ints(cu_q, "cu_q", seqs + 1, dev), _ints(cu_k, "cu_k", seqs + 1, dev), seqs, raw))
+    rc = lib.amoe_attn_prefill(
+        dev, d, _attn(scale, window, sinks, heads, dev), _rows(q, "q", n, d, dev), _rows(k, "k", m, d, dev),
+        _rows(v, "v", m, d, dev), _rows(out, "out", n, d, dev), n, m, _ints(cu_q, "cu_q", seqs + 1, dev),
+        _ints(cu_k, "cu_k", seqs + 1, dev), seqs, raw)
+    if rc:
+        _check(lib, rc)
     return out

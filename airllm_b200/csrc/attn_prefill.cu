@@ -133,6 +133,28 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Two float32 lanes in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t r) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // One warp finds the sequence and tile of CTA x: sequences in order, each one's last (longest) tile first.
 __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w) {
     const int lane = threadIdx.x % 32;
@@ -353,9 +375,12 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int i = 0; i < N; ++i)
                     if (i > last || i < first) s[i] = -INFINITY;
             }
-            float top = -INFINITY;
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // chains short enough to overlap
 #pragma unroll
-            for (int i = 0; i < N; ++i) top = fmaxf(top, s[i]);
+            for (int i = 0; i < N; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tops[e] = fmaxf(fmaxf(tops[e], s[i + 2 * e]), s[i + 2 * e + 1]);
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             const bool grown = (top - m) * p.scale_log2 > kLazy;
             bool waited = j == 0;
             if (__any_sync(0xffffffffu, grown)) {
@@ -380,16 +405,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                 m = mm;
             }
             const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
-            float sum = 0.0f;
+            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), off2 = pair(-off, -off);
+            uint64_t sums[2] = {0, 0};
 #pragma unroll
             for (int c = 0; c < N; c += 32) {
                 if (c >= cols) break;
                 uint32_t u[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float a = ex2(fmaf(s[c + 2 * i], p.scale_log2, -off));
-                    const float b = ex2(fmaf(s[c + 2 * i + 1], p.scale_log2, -off));
-                    sum += a + b;
+                    const float2 x = unpair(fma2(pair(s[c + 2 * i], s[c + 2 * i + 1]), scale2, off2));
+                    const float a = ex2(x.x), b = ex2(x.y);
+                    sums[i % 2] = add2(sums[i % 2], pair(a, b));
                     u[i] = pack2<TYPE>(a, b);
                 }
                 if (!waited) {  // the products of the tile before have read P
@@ -400,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 tmem_st16(tmem + lanes + C::kP + c / 2, u);
             }
             if (!ok) break;
-            l += sum;
+            const float2 sum = unpair(add2(sums[0], sums[1]));
+            l += sum.x + sum.y;
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
