@@ -36,8 +36,8 @@ using bs::tc_fence_after;
 using bs::tc_fence_before;
 
 constexpr int kRows = 128;
-constexpr int kSoftWarps = 4, kMmaWarp = 4, kTmaWarp = 5;
-constexpr int kThreads = 192;
+constexpr int kSoftWarps = 8, kFeedWarp = 8;
+constexpr int kThreads = 288;
 constexpr int kStages = 2;
 constexpr int kTmemCols = 256;
 constexpr float kLazy = 8.0f;  // log2 growth of a row's maximum that is left in the weights
@@ -56,7 +56,8 @@ struct Cfg {
     static constexpr int kHalves = D / 64;        // 128-byte column blocks of a row
     static constexpr int kQBytes = kRows * D * 2;
     static constexpr int kTileBytes = N * D * 2;
-    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + 256;
+    static constexpr int kSide = 256 + 64 + 2 * kRows * 4;  // barriers and work, votes, the half rows' exchange
+    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + kSide;
     static constexpr int kS = 0, kP = N, kO = N + N / 2;  // TMEM columns
     static_assert(kO + D <= kTmemCols, "TMEM columns");
 };
@@ -70,7 +71,16 @@ struct Work {
     int found;
 };
 
+// Waits for a phase, a second or so at most; at once when an earlier wait of the CTA gave up.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, Work *w) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*reinterpret_cast<volatile int *>(&w->dead)) return false;
     return bs::mbar_wait(bar, parity, &w->dead, 1);
 }
 
@@ -125,11 +135,38 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// C (32 or 64) columns of this warp's lanes, waited for in the same statement.
+template <int C>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[C]) {
+    if constexpr (C == 32) {
+        bs::tmem_ld32(taddr, v);
+    } else {
+        static_assert(C == 64, "32 or 64 columns");
+        uint32_t r[64];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,"
+            "%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+              "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+              "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+              "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+              "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+              "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+            : "r"(taddr)
+            : "memory");
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+    }
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));  // volatile: a run of them stays a run
     return y;
 }
 
@@ -236,11 +273,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *q_s = sm, *k_s = q_s + C::kQBytes, *v_s = k_s + kStages * C::kTileBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(v_s + kStages * C::kTileBytes);
-    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + kStages, *v_full = k_empty + kStages;
-    uint64_t *v_empty = v_full + kStages, *s_full = v_empty + kStages, *s_free = s_full + 1, *p_full = s_free + 1;
-    uint64_t *o_done = p_full + 1;
+    uint64_t *q_full = bars, *k_full = bars + 1, *v_full = k_full + kStages, *s_full = v_full + kStages;
+    uint64_t *s_free = s_full + 1, *p_full = s_free + 1, *o_done = p_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_done + 1);
     Work *work = reinterpret_cast<Work *>(tmem_slot + 1);
+    int *votes = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + 256);  // [2][kSoftWarps]
+    float *swap = reinterpret_cast<float *>(votes + 2 * kSoftWarps);                // [2][kRows]
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int kvh = blockIdx.y;
@@ -251,8 +289,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (threadIdx.x == 32) {
         mbar_init(q_full, 1);
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1);
-            mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+            mbar_init(k_full + i, 1), mbar_init(v_full + i, 1);
         }
         mbar_init(s_full, 1), mbar_init(o_done, 1);
         mbar_init(s_free, kSoftWarps), mbar_init(p_full, kSoftWarps);
@@ -260,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();
     if (!work->found) return;
-    if (warp == kMmaWarp) {
+    if (warp == kFeedWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "n"(kTmemCols)
                      : "memory");
@@ -275,24 +312,25 @@ __global__ void __launch_bounds__(kThreads, 2)
     // columns of the last tile that hold a visible key, in whole MMA steps
     const int last_cols = tiles > 0 ? (hi - lo - (tiles - 1) * N + 15) / 16 * 16 : 0;
 
-    if (warp == kTmaWarp) {
+    if (warp == kFeedWarp) {
+        // Copies and products.  A stage needs no barrier of its own to be refilled: S of tile j read (s_free)
+        // says that its Q K^T is done with K, and the weights of tile j written (p_full) that the
+        // products of tile j - 1 are done with V.
+        auto load = [&](uint8_t *ring, const CUtensorMap *tm, uint64_t *full, int j) {
+            const int s = j % kStages;
+            mbar_expect_tx(full + s, C::kTileBytes);
+            for (int h = 0; h < HALVES; ++h)
+                tma_3d(ring + s * C::kTileBytes + h * N * 128, tm, full + s, h * 64, kvh, k0 + lo + j * N);
+        };
         if (lane == 0 && tiles > 0) {
             mbar_expect_tx(q_full, p.tile_tokens * p.group * D * 2);
             for (int h = 0; h < HALVES; ++h) tma_3d(q_s + h * kRows * 128, &tm_q, q_full, h * 64, kvh * p.group, tok0);
-            for (int j = 0; j < tiles; ++j) {
-                const int s = j % kStages, row = k0 + lo + j * N;
-                const uint32_t ph = (uint32_t)(j / kStages - 1) & 1u;
-                if (j >= kStages && !wait_bar(k_empty + s, ph, work)) break;
-                mbar_expect_tx(k_full + s, C::kTileBytes);
-                for (int h = 0; h < HALVES; ++h)
-                    tma_3d(k_s + s * C::kTileBytes + h * N * 128, &tm_k, k_full + s, h * 64, kvh, row);
-                if (j >= kStages && !wait_bar(v_empty + s, ph, work)) break;
-                mbar_expect_tx(v_full + s, C::kTileBytes);
-                for (int h = 0; h < HALVES; ++h)
-                    tma_3d(v_s + s * C::kTileBytes + h * N * 128, &tm_v, v_full + s, h * 64, kvh, row);
+            for (int j = 0; j < kStages && j < tiles; ++j) {
+                load(k_s, &tm_k, k_full, j);
+                load(v_s, &tm_v, v_full, j);
             }
         }
-    } else if (warp == kMmaWarp) {
+        __syncwarp();
         const uint32_t q_a = smem_u32(q_s), k_a = smem_u32(k_s), v_a = smem_u32(v_s);
         bool ok = tiles > 0 && wait_warp(q_full, 0, work);
         for (int j = 0; ok && j <= tiles; ++j) {
@@ -311,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                                desc_sw128(k_a + s * C::kTileBytes + off * N * 128 + in, 16), id, i > 0);
                     }
                     mma_commit(s_full);
-                    mma_commit(k_empty + s);
+                    if (j > 0 && j - 1 + kStages < tiles) load(k_s, &tm_k, k_full, j - 1 + kStages);
                 }
                 __syncwarp();
             }
@@ -339,93 +377,97 @@ __global__ void __launch_bounds__(kThreads, 2)
                         mma_ts(tmem + C::kO, tmem + C::kP + i * 8,
                                desc_sw128(v_a + s * C::kTileBytes + i * 2048, N * 128), id, t > 0 || i > 0);
                     mma_commit(o_done);
-                    mma_commit(v_empty + s);
+                    if (t > 0 && t - 1 + kStages < tiles) load(v_s, &tm_v, v_full, t - 1 + kStages);
                 }
                 __syncwarp();
             }
         }
     } else {
-        // a thread's row: token r / group of the tile, query head r % group of the kv head
-        const int r = threadIdx.x, tok = r / p.group, head = kvh * p.group + r % p.group;
-        const int at = at0 + tok;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        // Two threads to a row, one for each half of a tile's keys: row r is token r / group of the tile, query
+        // head r % group of the kv head.  They agree on the maximum through their two warps' votes.
+        constexpr int H = N / 2;
+        const int r = threadIdx.x % kRows, half = threadIdx.x / kRows, tok = r / p.group;
+        const int head = kvh * p.group + r % p.group, at = at0 + tok;
+        const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(warp % 4 + 1) : "memory"); };
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;
+        bool ok = true;  // after a wait that gave up the warps go on to the end together, on what is there
         for (int j = 0; j < tiles; ++j) {
-            ok = wait_warp(s_full, (uint32_t)j & 1u, work);
-            if (!ok) break;
+            ok &= wait_warp(s_full, (uint32_t)j & 1u, work);
             tc_fence_after();
-            const int base = lo + j * N, cols = j + 1 == tiles ? last_cols : N;
-            float s[N];
-#pragma unroll
-            for (int c = 0; c < N; c += 32) {
-                if (c < cols) {
-                    bs::tmem_ld32(tmem + lanes + C::kS + c, *reinterpret_cast<float(*)[32]>(s + c));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c + i] = -INFINITY;
-                }
-            }
+            const int base = lo + j * N + half * H, cols = (j + 1 == tiles ? last_cols : N) - half * H;
+            float s[H];
+            tmem_ld<H>(tmem + lanes + C::kS + half * H, s);  // columns behind the tile's last are masked
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free);
-            if (base + N - 1 > at0 || (p.window > 0 && base <= hi - 1 - p.window)) {
+            if (base + H - 1 > at0 || (p.window > 0 && base <= hi - 1 - p.window)) {
                 const int last = at - base, first = p.window > 0 ? at - p.window + 1 - base : 0;
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+                for (int i = 0; i < H; ++i)
                     if (i > last || i < first) s[i] = -INFINITY;
             }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // chains short enough to overlap
 #pragma unroll
-            for (int i = 0; i < N; i += 8)
+            for (int i = 0; i < H; i += 8)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) tops[e] = fmaxf(fmaxf(tops[e], s[i + 2 * e]), s[i + 2 * e + 1]);
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            const bool grown = (top - m) * p.scale_log2 > kLazy;
-            bool waited = j == 0;
-            if (__any_sync(0xffffffffu, grown)) {
-                const float mm = fmaxf(m, top);
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            const bool grown = __any_sync(0xffffffffu, (top - m) * p.scale_log2 > kLazy);
+            int *vote = votes + (j & 1) * kSoftWarps;
+            if (lane == 0) vote[warp] = grown;
+            meet();
+            bool waited = j == 0;  // P and O are free once the products of the tile before are done
+            if (vote[warp] | vote[warp ^ 4]) {
+                swap[threadIdx.x] = top;
+                meet();
+                const float mm = fmaxf(m, fmaxf(top, swap[threadIdx.x ^ kRows]));
                 if (j > 0) {
-                    ok = wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
-                    if (!ok) break;
+                    ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
                     waited = true;
                     tc_fence_after();
                     const float keep = mm == -INFINITY ? 1.0f : ex2((m - mm) * p.scale_log2);
                     l *= keep;
 #pragma unroll
-                    for (int c = 0; c < D; c += 16) {
+                    for (int c = 0; c < D / 2; c += 16) {
                         float o[16];
-                        bs::tmem_ld16(tmem + lanes + C::kO + c, o);
+                        bs::tmem_ld16(tmem + lanes + C::kO + half * (D / 2) + c, o);
                         uint32_t u[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * keep);
-                        tmem_st16(tmem + lanes + C::kO + c, u);
+                        tmem_st16(tmem + lanes + C::kO + half * (D / 2) + c, u);
                     }
                 }
                 m = mm;
+                meet();  // the exchange is read before the next one
             }
             const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
             const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), off2 = pair(-off, -off);
             uint64_t sums[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < N; c += 32) {
-                if (c >= cols) break;
+            for (int c = 0; c < H; c += 32) {
+                if (c >= cols) continue;
                 uint32_t u[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 x = unpair(fma2(pair(s[c + 2 * i], s[c + 2 * i + 1]), scale2, off2));
-                    const float a = ex2(x.x), b = ex2(x.y);
-                    sums[i % 2] = add2(sums[i % 2], pair(a, b));
-                    u[i] = pack2<TYPE>(a, b);
+                for (int i = c; i < c + 32; i += 2) {
+                    const float2 x = unpair(fma2(pair(s[i], s[i + 1]), scale2, off2));
+                    s[i] = x.x, s[i + 1] = x.y;
                 }
-                if (!waited) {  // the products of the tile before have read P
-                    ok = wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
+#pragma unroll
+                for (int i = c; i < c + 32; ++i) s[i] = ex2(s[i]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sums[i % 2] = add2(sums[i % 2], pair(s[c + 2 * i], s[c + 2 * i + 1]));
+                    u[i] = pack2<TYPE>(s[c + 2 * i], s[c + 2 * i + 1]);
+                }
+                if (!waited) {
+                    ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
                     waited = true;
                     tc_fence_after();
                 }
-                tmem_st16(tmem + lanes + C::kP + c / 2, u);
+                tmem_st16(tmem + lanes + C::kP + (half * H + c) / 2, u);
             }
-            if (!ok) break;
+            if (!waited) ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
             const float2 sum = unpair(add2(sums[0], sums[1]));
             l += sum.x + sum.y;
             tmem_wait_st();
@@ -433,28 +475,30 @@ __global__ void __launch_bounds__(kThreads, 2)
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full);
         }
-        if (ok && tiles > 0) ok = wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
+        if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
+        swap[threadIdx.x] = l;
+        meet();
+        l += swap[threadIdx.x ^ kRows];
+        meet();
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
         const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
         if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - off);
         const float by = !ok ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
-        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
-        bool fine = true;
+        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + half * D;
+        float worst = 0.0f;  // 0, or NaN
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < D / 2; c += 32) {
             float o[32];
             __syncwarp();
             if (tiles > 0) {
-                bs::tmem_ld32(tmem + lanes + C::kO + c, o);
+                bs::tmem_ld32(tmem + lanes + C::kO + half * (D / 2) + c, o);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0.0f;
             }
-            float worst = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;  // 0, or NaN
-            fine &= worst == 0.0f;
+            for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;
             if (mine) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
@@ -465,12 +509,16 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
             }
         }
-        if (mine && ok && (!fine || !isfinite(l)))
+        __syncwarp();
+        swap[threadIdx.x] = worst;
+        meet();
+        worst += swap[threadIdx.x ^ kRows];
+        if (half == 0 && mine && ok && (worst != 0.0f || !isfinite(l)))
             row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kFeedWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols));
     }

@@ -8,9 +8,10 @@
 // c and s = cos, sin (angle) * concentration.  Angles of far positions lose float32, and a
 // value that lands next to a rounding border of the cache's type must fall on the side the
 // definition says, so angles, sines and products are float64 as in the reference, rounded
-// once to float32 (its stored type) and from there to the cache's.  One CTA takes one token:
-// d/2 threads compute the angles, then d/16 threads a head row turn eight pairs each with
-// the sines of their eight pairs in registers for every row they visit.
+// once to float32 (its stored type) and from there to the cache's.  A warp takes one token (four
+// warps, where there are few tokens): its lanes compute the angles, then d/16 lanes a head row turn eight
+// pairs each with the sines of their eight pairs in registers for every row they visit, the next
+// row's loads in flight.
 //
 // E4M3 rows: the scale is a power of two, so scaling is exact and only the rounding to E4M3
 // loses bits; the row's maximum is reduced over the d/16 lanes that hold it.
@@ -20,9 +21,9 @@ namespace amoe {
 namespace attn {
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 constexpr int kReadThreads = 256;
-constexpr int kReadTokens = 16;
+constexpr int kReadTokens = 4;
 constexpr int kNoRow = INT_MIN;  // in the place of a page: not a row of this call
 
 struct RopeDev {
@@ -35,7 +36,7 @@ struct AppendParams {
     CacheDev c;
     RowsDev q, k, v, q_out, k_out, v_out;
     const int32_t *cu, *past;
-    int tokens, seqs, q_heads, q_out_type, k_out_type, v_out_type;
+    int tokens, seqs, q_heads, q_out_type, k_out_type, v_out_type, warps;  // warps to a token
     RopeDev rope;
 };
 
@@ -106,65 +107,80 @@ __device__ __forceinline__ void cache_store(char *pages, uint8_t *scales, int64_
 template <int D, int SRC, int CACHE>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int L = D / 16;  // lanes of a row
+    constexpr int STEP = 32 / L;  // rows of a warp at a time
     constexpr int ES = SRC == AMOE_GGUF_F32 ? 4 : 2;
-    __shared__ double2 cs[D / 2];
-    const int t = blockIdx.x;
-    const int last = p.cu[p.seqs];
-    if (t >= last) return;
+    __shared__ double2 cs_all[kAppendThreads / 32][D / 2];
+    const int lane = threadIdx.x % 32, part = lane % L;
+    double2 *cs = cs_all[threadIdx.x / 32];
+    const int64_t warp = (int64_t)blockIdx.x * (kAppendThreads / 32) + threadIdx.x / 32;
+    const int t = (int)(warp / p.warps), r0 = (int)(warp % p.warps) * STEP + lane / L;
+    if (t >= p.tokens || t >= p.cu[p.seqs]) return;
+    const int rows = p.q_heads + 2 * p.c.heads;
+
+    struct Row {
+        float a[8], b[8];
+    };
+    auto load = [&](int r, Row &x) {
+        if (r >= rows) return;
+        const bool is_q = r < p.q_heads, is_k = !is_q && r < p.q_heads + p.c.heads;
+        const RowsDev &src = is_q ? p.q : is_k ? p.k : p.v;
+        const int h = is_q ? r : is_k ? r - p.q_heads : r - p.q_heads - p.c.heads;
+        const char *at = src.p + t * src.ts + h * src.hs + part * 8 * ES;
+        load8<SRC>(at, x.a);
+        load8<SRC>(at + D / 2 * ES, x.b);
+    };
+    Row next{};
+    load(r0, next);  // on its way while the position and its sines are found
+
     const int s = find_seq(p.cu, p.seqs, t);
     const int start = p.cu[s], past = p.past[s];
     if (start > t || start < 0 || p.cu[s + 1] <= t || past < 0) {
-        if (threadIdx.x == 0) atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
+        if (lane == 0) atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
         return;
     }
     const int64_t pos = (int64_t)past + (t - start);
-    if (p.rope.on && threadIdx.x < D / 2) {
-        double sn, c;
-        sincos((double)pos * p.rope.freq[threadIdx.x], &sn, &c);
-        cs[threadIdx.x] = make_double2(c * p.rope.conc, sn * p.rope.conc);
-    }
     const int page = page_of(p.c, s, pos);
-    __syncthreads();
-
-    const int part = threadIdx.x % L;
     double2 w[8];
     if (p.rope.on) {
 #pragma unroll
+        for (int i = lane; i < D / 2; i += 32) {
+            double sn, c;
+            sincos((double)pos * p.rope.freq[i], &sn, &c);
+            cs[i] = make_double2(c * p.rope.conc, sn * p.rope.conc);
+        }
+        __syncwarp();
+#pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = cs[part * 8 + i];
     }
-    const int rows = p.q_heads + 2 * p.c.heads;
-    // whole warps stay together for the row maximum's shuffles: the bound is rounded up
-    for (int r0 = 0; r0 < rows; r0 += kAppendThreads / L) {
-        const int r = r0 + threadIdx.x / L;
+
+    // the warp stays together for the row maximum's shuffles: the bound is the warp's first row
+    for (int r = r0; r - lane / L < rows; r += STEP * p.warps) {
+        Row x = next;
+        load(r + STEP * p.warps, next);
         const bool live = r < rows;
         const bool is_q = r < p.q_heads, is_k = !is_q && r < p.q_heads + p.c.heads;
         const int h = is_q ? r : is_k ? r - p.q_heads : r - p.q_heads - p.c.heads;
-        float a[8] = {}, b[8] = {};
-        if (live) {
-            const RowsDev &src = is_q ? p.q : is_k ? p.k : p.v;
-            const char *x = src.p + t * src.ts + h * src.hs + part * 8 * ES;
-            load8<SRC>(x, a);
-            load8<SRC>(x + D / 2 * ES, b);
-            if (p.rope.on && (is_q || is_k)) {
+        if (p.rope.on && live && (is_q || is_k)) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const double f = a[i], g = b[i];
-                    a[i] = (float)(f * w[i].x - g * w[i].y);
-                    b[i] = (float)(g * w[i].x + f * w[i].y);
-                }
-            }
-            const RowsDev &dst = is_q ? p.q_out : is_k ? p.k_out : p.v_out;
-            if (dst.p) {
-                const int type = is_q ? p.q_out_type : is_k ? p.k_out_type : p.v_out_type;
-                const int es = elem_size(type);
-                char *y = dst.p + t * dst.ts + h * dst.hs + part * 8 * es;
-                store8_any(y, type, a);
-                store8_any(y + D / 2 * es, type, b);
+            for (int i = 0; i < 8; ++i) {
+                const double f = x.a[i], g = x.b[i];
+                x.a[i] = (float)(f * w[i].x - g * w[i].y);
+                x.b[i] = (float)(g * w[i].x + f * w[i].y);
             }
         }
+        const RowsDev &dst = is_q ? p.q_out : is_k ? p.k_out : p.v_out;
+        if (live && dst.p) {
+            const int type = is_q ? p.q_out_type : is_k ? p.k_out_type : p.v_out_type;
+            const int es = elem_size(type);
+            char *y = dst.p + t * dst.ts + h * dst.hs + part * 8 * es;
+            store8_any(y, type, x.a);
+            store8_any(y + D / 2 * es, type, x.b);
+        }
         const bool write = live && !is_q && page >= 0;
-        const int64_t row = write ? cache_row(p.c, page, h, pos) : 0;
-        cache_store<D, CACHE>(is_k ? p.c.k : p.c.v, is_k ? p.c.ks : p.c.vs, row, part, a, b, write);
+        if (__any_sync(0xffffffffu, write)) {
+            const int64_t row = write ? cache_row(p.c, page, h, pos) : 0;
+            cache_store<D, CACHE>(is_k ? p.c.k : p.c.v, is_k ? p.c.ks : p.c.vs, row, part, x.a, x.b, write);
+        }
     }
 }
 
@@ -175,69 +191,80 @@ struct ReadParams {
     int tokens, seqs, k_type, v_type;
 };
 
+// A warp takes four rows of the output; its lanes walk (head, token) pairs, token first: four
+// tokens of a head are one run of the page, and a lane moves 16 bytes of it.
 template <int D, int CACHE>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ ReadParams p) {
-    constexpr int C = D / 8;  // eight elements an item
-    __shared__ int page[kReadTokens];
-    __shared__ int64_t pos[kReadTokens];
-    const int t0 = blockIdx.x * kReadTokens;
+    constexpr int E = CACHE == AMOE_KV_E4M3 ? 16 : 8;  // elements of 16 bytes
+    constexpr int C = D / E, RPI = 32 / C;             // lanes of a row, rows at a time
+    const int lane = threadIdx.x % 32, ch = lane % C;
+    const int64_t first_row = ((int64_t)blockIdx.x * (kReadThreads / 32) + threadIdx.x / 32) * kReadTokens;
     const int last = min(p.cu[p.seqs], p.tokens);
-    if (t0 >= last) return;
-    if (threadIdx.x < kReadTokens) {
-        const int t = t0 + threadIdx.x;
-        int pg = kNoRow;
-        int64_t at = 0;
-        if (t < last) {
-            const int s = find_seq(p.cu, p.seqs, t);
-            const int start = p.cu[s];
-            const int64_t f = p.first ? p.first[s] : 0;
-            if (start < 0 || start > t || p.cu[s + 1] <= t || f < 0) {
-                atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
-            } else {
-                at = f + (t - start);
-                pg = page_of(p.c, s, at);
-            }
+    if (first_row >= last) return;
+    const int t0 = (int)first_row;
+    int page = kNoRow;
+    int64_t pos = 0;
+    if (lane < kReadTokens && t0 + lane < last) {
+        const int t = t0 + lane;
+        const int s = find_seq(p.cu, p.seqs, t);
+        const int start = p.cu[s];
+        const int64_t f = p.first ? p.first[s] : 0;
+        if (start < 0 || start > t || p.cu[s + 1] <= t || f < 0) {
+            atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
+        } else {
+            pos = f + (t - start);
+            page = page_of(p.c, s, pos);
         }
-        page[threadIdx.x] = pg;
-        pos[threadIdx.x] = at;
     }
-    __syncthreads();
-    const int per = p.c.heads * C;  // items of one token's keys or values
-    for (int i = threadIdx.x; i < kReadTokens * 2 * per; i += kReadThreads) {
-        const int tok = i / (2 * per), j = i % (2 * per);
-        const bool is_v = j >= per;
-        const int h = (j % per) / C, ch = j % C;
-        const int pg = page[tok];
-        if (pg == kNoRow) continue;
-        float x[8] = {};
+    __syncwarp();
+    // row of a head's first page slot, in the pages: the head only adds a multiple of the page size
+    const int64_t row0 = page >= 0 ? cache_row(p.c, page, 0, pos) : 0;
+#pragma unroll 4
+    for (int i = lane / C; i - lane / C < kReadTokens * 2 * p.c.heads; i += RPI) {
+        const int tok = i % kReadTokens;
+        const int pg = __shfl_sync(0xffffffffu, page, tok);
+        const int64_t base = __shfl_sync(0xffffffffu, row0, tok);
+        const int hk = i / kReadTokens;
+        if (hk >= 2 * p.c.heads || pg == kNoRow) continue;
+        const bool is_v = hk >= p.c.heads;
+        const int h = is_v ? hk - p.c.heads : hk;
+        float x[E] = {};
         if (pg >= 0) {
-            const int64_t row = cache_row(p.c, pg, h, pos[tok]);
-            const char *src = is_v ? p.c.v : p.c.k;
+            const int64_t row = base + ((int64_t)h << p.c.shift);
+            const char *src = (is_v ? p.c.v : p.c.k) + row * (D * 16 / E) + ch * 16;
             if constexpr (CACHE == AMOE_KV_E4M3) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(src + row * D + ch * 8);
+                const uint4 w = *reinterpret_cast<const uint4 *>(src);
                 const float by = e8m0_to_float((is_v ? p.c.vs : p.c.ks)[row]);
-                const uint32_t u[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    const uint32_t hh = e4m3x2_to_f16x2(u[m]);
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hh));
-                    x[2 * m] = f.x * by, x[2 * m + 1] = f.y * by;
+                    uint32_t lo, hi;
+                    e4m3x4_to_f16x2(u[m], lo, hi);
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
+                    const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                    x[4 * m] = f.x * by, x[4 * m + 1] = f.y * by, x[4 * m + 2] = g.x * by, x[4 * m + 3] = g.y * by;
                 }
             } else {
-                load8<CACHE>(src + (row * D + ch * 8) * 2, x);
+                load8<CACHE>(src, x);
             }
         }
         const RowsDev &dst = is_v ? p.v : p.k;
         const int type = is_v ? p.v_type : p.k_type;
-        store8_any(dst.p + (int64_t)(t0 + tok) * dst.ts + h * dst.hs + ch * 8 * elem_size(type), type, x);
+        char *y = dst.p + (int64_t)(t0 + tok) * dst.ts + h * dst.hs + ch * E * elem_size(type);
+#pragma unroll
+        for (int m = 0; m < E; m += 8)
+            store8_any(y + m * elem_size(type), type, *reinterpret_cast<const float(*)[8]>(x + m));
     }
 }
 
 template <int D, int SRC>
 cudaError_t launch_append(const AppendParams &p, int cache, cudaStream_t st) {
-    if (cache == AMOE_GGUF_F16) append_kernel<D, SRC, AMOE_GGUF_F16><<<p.tokens, kAppendThreads, 0, st>>>(p);
-    else if (cache == AMOE_GGUF_BF16) append_kernel<D, SRC, AMOE_GGUF_BF16><<<p.tokens, kAppendThreads, 0, st>>>(p);
-    else append_kernel<D, SRC, AMOE_KV_E4M3><<<p.tokens, kAppendThreads, 0, st>>>(p);
+    const int64_t warps = (int64_t)p.tokens * p.warps;
+    if (warps > INT_MAX) return cudaErrorInvalidValue;
+    const int grid = (int)((warps - 1) / (kAppendThreads / 32) + 1);
+    if (cache == AMOE_GGUF_F16) append_kernel<D, SRC, AMOE_GGUF_F16><<<grid, kAppendThreads, 0, st>>>(p);
+    else if (cache == AMOE_GGUF_BF16) append_kernel<D, SRC, AMOE_GGUF_BF16><<<grid, kAppendThreads, 0, st>>>(p);
+    else append_kernel<D, SRC, AMOE_KV_E4M3><<<grid, kAppendThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -250,7 +277,7 @@ cudaError_t launch_append_d(const AppendParams &p, int src, int cache, cudaStrea
 
 template <int D>
 cudaError_t launch_read_d(const ReadParams &p, int cache, cudaStream_t st) {
-    const int grid = (p.tokens - 1) / kReadTokens + 1;
+    const int grid = (p.tokens - 1) / (kReadTokens * kReadThreads / 32) + 1;
     if (cache == AMOE_GGUF_F16) read_kernel<D, AMOE_GGUF_F16><<<grid, kReadThreads, 0, st>>>(p);
     else if (cache == AMOE_GGUF_BF16) read_kernel<D, AMOE_GGUF_BF16><<<grid, kReadThreads, 0, st>>>(p);
     else read_kernel<D, AMOE_KV_E4M3><<<grid, kReadThreads, 0, st>>>(p);
@@ -319,6 +346,8 @@ int amoe_kv_append(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const i
     p.q_out_type = q_out ? q_out->type : 0;
     p.k_out_type = k_out ? k_out->type : 0;
     p.v_out_type = v_out ? v_out->type : 0;
+    // few tokens: more warps to each, for the latency (each finds the sines again)
+    p.warps = tokens < 148 * 8 ? 4 : 1;
     if (rope) {
         for (int i = 0; i < D / 2; ++i) p.rope.freq[i] = rope->freq[i];
         p.rope.conc = rope->concentration;
