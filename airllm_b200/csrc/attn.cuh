@@ -47,6 +47,25 @@ __host__ __device__ inline int find_seq(const int32_t *cu, int seqs, int t) {
     return lo;
 }
 
+// The same for N rows t, t + 1, ... by a whole warp, a load for every 32 sequences instead of a chain of them.
+// Starts that decrease give some sequence in [0, seqs) here too; the caller checks that it holds the row.
+template <int N>
+__device__ __forceinline__ void find_seqs(const int32_t *cu, int seqs, int t, int (&s)[N]) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = 0;
+    for (int s0 = 0; s0 < seqs; s0 += 32) {
+        const int end = s0 + lane < seqs ? cu[s0 + lane + 1] : INT_MAX;
+        uint32_t behind = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            behind = __ballot_sync(0xffffffffu, end <= t + k);
+            s[k] = min(s[k] + __popc(behind), seqs - 1);
+        }
+        if (behind != 0xffffffffu) break;  // the last row's sequence, and so every one's, is found
+    }
+}
+
 // Page of position pos (>= 0) of sequence s, or the negated status bit where the table has none.
 __host__ __device__ inline int lookup_page(const CacheDev &c, int s, int64_t pos) {
     const int64_t i = pos >> c.shift;
