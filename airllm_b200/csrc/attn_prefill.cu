@@ -36,10 +36,6 @@ using bs::tc_fence_after;
 using bs::tc_fence_before;
 
 constexpr int kRows = 128;
-constexpr int kSoftWarps = 8, kFeedWarp = 8;
-constexpr int kThreads = 288;
-constexpr int kStages = 2;
-constexpr int kTmemCols = 256;
 constexpr float kLazy = 8.0f;  // log2 growth of a row's maximum that is left in the weights
 
 struct PrefillParams {
@@ -47,19 +43,26 @@ struct PrefillParams {
     const int32_t *cu_q, *cu_k;
     const float *sinks;
     float scale_log2;
-    int window, q_tokens, k_tokens, seqs, group, tile_tokens;
+    int window, q_tokens, k_tokens, seqs, group, tile_tokens, kv_heads;
 };
 
 template <int D>
 struct Cfg {
-    static constexpr int N = D == 64 ? 128 : 64;  // keys of a tile
+    static constexpr int N = 64;                  // keys of a tile
     static constexpr int kHalves = D / 64;        // 128-byte column blocks of a row
+    static constexpr int kStages = 2;
     static constexpr int kQBytes = kRows * D * 2;
     static constexpr int kTileBytes = N * D * 2;
+    static constexpr int kCtas = D == 64 ? 3 : 2;  // to an SM
+    static constexpr int kSplit = D == 64 ? 1 : 2;  // threads to a row
+    static constexpr int kSoftWarps = 4 * kSplit, kFeedWarp = kSoftWarps, kThreads = 32 * (kSoftWarps + 1);
     static constexpr int kSide = 256 + 64 + 2 * kRows * 4;  // barriers and work, votes, the half rows' exchange
     static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + kSide;
-    static constexpr int kS = 0, kP = N, kO = N + N / 2;  // TMEM columns
-    static_assert(kO + D <= kTmemCols, "TMEM columns");
+    // TMEM columns: S and O in one allocation (powers of two), P in another where three CTAs share the SM
+    static constexpr int kTmemCols = D == 64 ? 128 : 256, kTmemP = D == 64 ? 32 : 0;
+    static constexpr int kS = 0, kO = N, kP = D == 64 ? 0 : N + D;
+    static_assert(kO + D + (kTmemP ? 0 : N / 2) <= kTmemCols && kCtas * (kTmemCols + kTmemP) <= 512, "TMEM columns");
+    static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 // What a CTA works on, found by one warp and shared.
@@ -121,6 +124,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
                  "r"(a), "l"(b), "r"(id), "r"((uint32_t)add)
                  : "memory");
 }
+// One lane of a converged warp.  The compiler knows what elect.sync picks to be one thread and keeps
+// descriptors in uniform registers; behind `lane == 0` an MMA took 100 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+    return e != 0;
+}
+
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
@@ -228,26 +239,31 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w
     return false;
 }
 
-// A row again, key by visible key: for results that are not finite.
+// A row again, key by visible key: for results that are not finite.  Its arrays stay in local memory (no loop is
+// unrolled), so that the path costs the kernel no registers.
 template <int D, int TYPE>
-__device__ __noinline__ void row_again(const PrefillParams &p, int tok, int head, int k0, int from, int at) {
-    float acc[D], q[D], m = -INFINITY, l = 0.0f;
+__device__ __forceinline__ void row_again(const PrefillParams &p, int tok, int head, int k0, int from, int at) {
+    float acc[D], m = -INFINITY, l = 0.0f;
     const int kvh = head / p.group;
-    for (int d = 0; d < D; d += 8) {
-        load8<TYPE>(p.q.p + tok * p.q.ts + head * p.q.hs + d * 2, *reinterpret_cast<float(*)[8]>(q + d));
-        for (int i = 0; i < 8; ++i) acc[d + i] = 0.0f;
-    }
+    const char *q = p.q.p + tok * p.q.ts + head * p.q.hs;
+    float x[8], y[8];
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) acc[d] = 0.0f;
+#pragma unroll 1
     for (int j = from; j <= at; ++j) {
         const char *k = p.k.p + (k0 + j) * p.k.ts + kvh * p.k.hs, *v = p.v.p + (k0 + j) * p.v.ts + kvh * p.v.hs;
-        float x[8], dot = 0.0f;
+        float dot = 0.0f;
+#pragma unroll 1
         for (int d = 0; d < D; d += 8) {
-            load8<TYPE>(k + d * 2, x);
-            for (int i = 0; i < 8; ++i) dot = fmaf(q[d + i], x[i], dot);
+            load8<TYPE>(q + d * 2, x);
+            load8<TYPE>(k + d * 2, y);
+            for (int i = 0; i < 8; ++i) dot = fmaf(x[i], y[i], dot);
         }
         const float s = dot * p.scale_log2, mm = fmaxf(m, s), z = mm == -INFINITY ? 0.0f : mm;
         const float keep = exp2f(m - z), e = exp2f(s - z);
         m = mm;
         l = l * keep + e;
+#pragma unroll 1
         for (int d = 0; d < D; d += 8) {
             load8<TYPE>(v + d * 2, x);
             for (int i = 0; i < 8; ++i) acc[d + i] = acc[d + i] * keep + e * x[i];
@@ -256,19 +272,19 @@ __device__ __noinline__ void row_again(const PrefillParams &p, int tok, int head
     const float z = m == -INFINITY ? 0.0f : m;
     if (p.sinks) l += exp2f(p.sinks[head] * kLog2e - z);
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
     for (int d = 0; d < D; d += 8) {
-        float x[8];
         for (int i = 0; i < 8; ++i) x[i] = acc[d + i] * by;
         store8<TYPE>(p.out.p + tok * p.out.ts + head * p.out.hs + d * 2, x);
     }
 }
 
 template <int D, int TYPE>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
     prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
     using C = Cfg<D>;
-    constexpr int N = C::N, HALVES = C::kHalves;
+    constexpr int N = C::N, HALVES = C::kHalves, kStages = C::kStages, kFeedWarp = C::kFeedWarp, kSoftWarps = C::kSoftWarps;
     extern __shared__ __align__(1024) uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *q_s = sm, *k_s = q_s + C::kQBytes, *v_s = k_s + kStages * C::kTileBytes;
@@ -276,14 +292,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint64_t *q_full = bars, *k_full = bars + 1, *v_full = k_full + kStages, *s_full = v_full + kStages;
     uint64_t *s_free = s_full + 1, *p_full = s_free + 1, *o_done = p_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_done + 1);
-    Work *work = reinterpret_cast<Work *>(tmem_slot + 1);
+    Work *work = reinterpret_cast<Work *>(tmem_slot + 2);
     int *votes = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + 256);  // [2][kSoftWarps]
     float *swap = reinterpret_cast<float *>(votes + 2 * kSoftWarps);                // [2][kRows]
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int kvh = blockIdx.y;
+    const int kvh = blockIdx.x % p.kv_heads;
     if (warp == 0) {
-        const bool f = find_work(p, blockIdx.x, work);
+        const bool f = find_work(p, blockIdx.x / p.kv_heads, work);
         if (lane == 0) work->found = f;
     }
     if (threadIdx.x == 32) {
@@ -299,14 +315,18 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!work->found) return;
     if (warp == kFeedWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "n"(kTmemCols)
+                     "n"(C::kTmemCols)
                      : "memory");
+        if (C::kTmemP)
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot + 1)),
+                         "n"(C::kTmemP ? C::kTmemP : 32)
+                         : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = *tmem_slot, tmem_p = C::kTmemP ? tmem_slot[1] : tmem + C::kP;
     const int tok0 = work->tok0, at0 = work->at0, lo = work->lo, hi = work->hi, k0 = work->k0;
     const int tiles = hi > lo ? (hi - lo - 1) / N + 1 : 0;
     // columns of the last tile that hold a visible key, in whole MMA steps
@@ -331,32 +351,32 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
         __syncwarp();
-        const uint32_t q_a = smem_u32(q_s), k_a = smem_u32(k_s), v_a = smem_u32(v_s);
+        const uint64_t q_d = desc_sw128(smem_u32(q_s), 16), k_d = desc_sw128(smem_u32(k_s), 16);
+        const uint64_t v_d = desc_sw128(smem_u32(v_s), N * 128);
         bool ok = tiles > 0 && wait_warp(q_full, 0, work);
-        for (int j = 0; ok && j <= tiles; ++j) {
-            if (j < tiles) {  // S = Q K^T of tile j
+        auto scores = [&](int j) {  // S = Q K^T of tile j
+            if (j >= tiles) return;
                 const int s = j % kStages;
                 ok = wait_warp(k_full + s, (uint32_t)(j / kStages) & 1u, work);
                 if (ok && j > 0) ok = wait_warp(s_free, (uint32_t)(j - 1) & 1u, work);
-                if (!ok) break;
+                if (!ok) return;
                 tc_fence_after();
-                if (lane == 0) {
+                if (elect_one()) {
                     const uint32_t id = idesc<TYPE>(j + 1 == tiles ? last_cols : N, false);
+                    const uint64_t kd = k_d + s * (C::kTileBytes / 16);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t off = i / 4, in = i % 4 * 32;
-                        mma_ss(tmem + C::kS, desc_sw128(q_a + off * kRows * 128 + in, 16),
-                               desc_sw128(k_a + s * C::kTileBytes + off * N * 128 + in, 16), id, i > 0);
-                    }
+                    for (int i = 0; i < D / 16; ++i)
+                        mma_ss(tmem + C::kS, q_d + i / 4 * (kRows * 8) + i % 4 * 2, kd + i / 4 * (N * 8) + i % 4 * 2, id, i > 0);
                     mma_commit(s_full);
                     if (j > 0 && j - 1 + kStages < tiles) load(k_s, &tm_k, k_full, j - 1 + kStages);
                 }
                 __syncwarp();
-            }
-            if (j > 0) {  // O += P V of tile j - 1
-                const int t = j - 1, s = t % kStages;
+        };
+        auto weigh = [&](int t) {  // O += P V of tile t
+            if (t < 0 || !ok) return;
+                const int s = t % kStages;
                 ok = wait_warp(v_full + s, (uint32_t)(t / kStages) & 1u, work);
-                if (!ok) break;
+                if (!ok) return;
                 const int cols = t + 1 == tiles ? last_cols : N;
                 const int seen = hi - lo - t * N;
                 if (seen < cols) {  // no value behind the last visible key reaches the products
@@ -369,27 +389,33 @@ __global__ void __launch_bounds__(kThreads, 2)
                     __syncwarp();
                 }
                 ok = wait_warp(p_full, (uint32_t)t & 1u, work);
-                if (!ok) break;
+                if (!ok) return;
                 tc_fence_after();
-                if (lane == 0) {
+                if (elect_one()) {
                     const uint32_t id = idesc<TYPE>(D, true);
-                    for (int i = 0; i < cols / 16; ++i)
-                        mma_ts(tmem + C::kO, tmem + C::kP + i * 8,
-                               desc_sw128(v_a + s * C::kTileBytes + i * 2048, N * 128), id, t > 0 || i > 0);
+                    const uint64_t vd = v_d + s * (C::kTileBytes / 16);
+#pragma unroll
+                    for (int i = 0; i < N / 16; ++i)
+                        if (i * 16 < cols) mma_ts(tmem + C::kO, tmem_p + i * 8, vd + i * 128, id, t > 0 || i > 0);
                     mma_commit(o_done);
                     if (t > 0 && t - 1 + kStages < tiles) load(v_s, &tm_v, v_full, t - 1 + kStages);
                 }
                 __syncwarp();
-            }
+        };
+        for (int j = 0; ok && j <= tiles; ++j) {
+            scores(j);
+            weigh(j - 1);
         }
     } else {
-        // Two threads to a row, one for each half of a tile's keys: row r is token r / group of the tile, query
-        // head r % group of the kv head.  They agree on the maximum through their two warps' votes.
-        constexpr int H = N / 2;
-        const int r = threadIdx.x % kRows, half = threadIdx.x / kRows, tok = r / p.group;
+        // Row r is token r / group of the tile, query head r % group of the kv head.  Where two threads share a
+        // row, each takes half of a tile's keys and they agree on the maximum through their two warps' votes.
+        constexpr int SPLIT = C::kSplit, H = N / SPLIT;
+        const int r = threadIdx.x % kRows, half = SPLIT == 2 ? threadIdx.x / kRows : 0, tok = r / p.group;
         const int head = kvh * p.group + r % p.group, at = at0 + tok;
         const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(warp % 4 + 1) : "memory"); };
+        auto meet = [&]() {
+            if constexpr (SPLIT == 2) asm volatile("bar.sync %0, 64;" ::"r"(warp % 4 + 1) : "memory");
+        };
         float m = -INFINITY, l = 0.0f;
         bool ok = true;  // after a wait that gave up the warps go on to the end together, on what is there
         for (int j = 0; j < tiles; ++j) {
@@ -414,28 +440,37 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int e = 0; e < 4; ++e) tops[e] = fmaxf(fmaxf(tops[e], s[i + 2 * e]), s[i + 2 * e + 1]);
             float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             const bool grown = __any_sync(0xffffffffu, (top - m) * p.scale_log2 > kLazy);
-            int *vote = votes + (j & 1) * kSoftWarps;
-            if (lane == 0) vote[warp] = grown;
-            meet();
-            bool waited = j == 0;  // P and O are free once the products of the tile before are done
-            if (vote[warp] | vote[warp ^ 4]) {
-                swap[threadIdx.x] = top;
+            bool any = grown;
+            if constexpr (SPLIT == 2) {
+                int *vote = votes + (j & 1) * kSoftWarps;
+                if (lane == 0) vote[warp] = grown;
                 meet();
-                const float mm = fmaxf(m, fmaxf(top, swap[threadIdx.x ^ kRows]));
+                any = vote[warp] | vote[warp ^ 4];
+            }
+            bool waited = j == 0;  // P and O are free once the products of the tile before are done
+            if (any) {
+                if constexpr (SPLIT == 2) {
+                    swap[threadIdx.x] = top;
+                    meet();
+                    top = fmaxf(top, swap[threadIdx.x ^ kRows]);
+                }
+                const float mm = fmaxf(m, top);
                 if (j > 0) {
-                    ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
+                    if (!waited) {
+                        ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
+                        tc_fence_after();
+                    }
                     waited = true;
-                    tc_fence_after();
                     const float keep = mm == -INFINITY ? 1.0f : ex2((m - mm) * p.scale_log2);
                     l *= keep;
 #pragma unroll
-                    for (int c = 0; c < D / 2; c += 16) {
+                    for (int c = 0; c < D / SPLIT; c += 16) {
                         float o[16];
-                        bs::tmem_ld16(tmem + lanes + C::kO + half * (D / 2) + c, o);
+                        bs::tmem_ld16(tmem + lanes + C::kO + half * (D / SPLIT) + c, o);
                         uint32_t u[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * keep);
-                        tmem_st16(tmem + lanes + C::kO + half * (D / 2) + c, u);
+                        tmem_st16(tmem + lanes + C::kO + half * (D / SPLIT) + c, u);
                     }
                 }
                 m = mm;
@@ -465,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     waited = true;
                     tc_fence_after();
                 }
-                tmem_st16(tmem + lanes + C::kP + (half * H + c) / 2, u);
+                tmem_st16(tmem_p + lanes + (half * H + c) / 2, u);
             }
             if (!waited) ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
             const float2 sum = unpair(add2(sums[0], sums[1]));
@@ -477,22 +512,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
-        swap[threadIdx.x] = l;
-        meet();
-        l += swap[threadIdx.x ^ kRows];
-        meet();
+        if constexpr (SPLIT == 2) {
+            swap[threadIdx.x] = l;
+            meet();
+            l += swap[threadIdx.x ^ kRows];
+            meet();
+        }
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
         const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
         if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - off);
         const float by = !ok ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
-        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + half * D;
+        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + half * (D / SPLIT) * 2;
         float worst = 0.0f;  // 0, or NaN
 #pragma unroll
-        for (int c = 0; c < D / 2; c += 32) {
+        for (int c = 0; c < D / SPLIT; c += 32) {
             float o[32];
             __syncwarp();
             if (tiles > 0) {
-                bs::tmem_ld32(tmem + lanes + C::kO + half * (D / 2) + c, o);
+                bs::tmem_ld32(tmem + lanes + C::kO + half * (D / SPLIT) + c, o);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0.0f;
@@ -510,9 +547,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
         __syncwarp();
-        swap[threadIdx.x] = worst;
-        meet();
-        worst += swap[threadIdx.x ^ kRows];
+        if constexpr (SPLIT == 2) {
+            swap[threadIdx.x] = worst;
+            meet();
+            worst += swap[threadIdx.x ^ kRows];
+        }
         if (half == 0 && mine && ok && (worst != 0.0f || !isfinite(l)))
             row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
     }
@@ -520,7 +559,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     if (warp == kFeedWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kTmemCols));
+        if (C::kTmemP)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_p),
+                         "n"(C::kTmemP ? C::kTmemP : 32));
     }
 }
 
@@ -550,7 +592,7 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_release);
     }
-    kernel<<<grid, kThreads, Cfg<D>::kSmem, st>>>(q, k, v, p);
+    kernel<<<grid, Cfg<D>::kThreads, Cfg<D>::kSmem, st>>>(q, k, v, p);
     return cudaGetLastError();
 }
 
@@ -576,7 +618,6 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     if (int rc = check_group(q->heads, k->heads)) return rc;
     if (!cu_q || !cu_k) return reject("cu_q and cu_k must not be NULL");
     if (seqs < 1) return reject("seqs must be positive");
-    if (k->heads > 65535) return reject("more than 65535 kv heads in one prefill call");
     if (device < 0 || device >= kMaxDevices) return reject("device ordinal out of range");
     if (q_tokens == 0) return AMOE_OK;
     PrefillParams p{};
@@ -587,9 +628,10 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     p.window = attn->window, p.q_tokens = q_tokens, p.k_tokens = k_tokens, p.seqs = seqs;
     p.group = q->heads / k->heads;
     p.tile_tokens = kRows / p.group;
+    p.kv_heads = k->heads;
     // every sequence's last tile may be a short one
-    const int64_t tiles = (int64_t)q_tokens / p.tile_tokens + (seqs < q_tokens ? seqs : q_tokens);
-    if (tiles > INT_MAX) return reject("too many query rows");
+    const int64_t ctas = ((int64_t)q_tokens / p.tile_tokens + (seqs < q_tokens ? seqs : q_tokens)) * k->heads;
+    if (ctas > INT_MAX) return reject("too many query rows");
     DeviceScope scope;
     cudaError_t e = scope.enter(device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
@@ -603,7 +645,7 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
         !encode_rows(&tk, k, head_dim, k_tokens, 1, n) || !encode_rows(&tv, v, head_dim, k_tokens, 1, n))
         return reject("prefill: strides of q, k or v that a tensor map cannot take");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)tiles, k->heads);
+    const dim3 grid((unsigned)ctas);  // kv heads first, then a sequence's tiles from the longest down
     if (head_dim == 64)
         e = q->type == AMOE_GGUF_F16 ? launch<64, AMOE_GGUF_F16>(tq, tk, tv, p, device, grid, st)
                                      : launch<64, AMOE_GGUF_BF16>(tq, tk, tv, p, device, grid, st);
