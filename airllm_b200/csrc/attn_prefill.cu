@@ -55,6 +55,9 @@ struct Cfg {
     static constexpr int kTileBytes = N * D * 2;
     static constexpr int kCtas = D == 64 ? 3 : 2;  // to an SM
     static constexpr int kSplit = D == 64 ? 1 : 2;  // threads to a row
+    // One pair of exponentials in eight on the FMA pipe.  8192 tokens of 64 heads: 733 us with none, 704 with one
+    // in eight, 713 with one in four; 128-wide heads, whose products bound them, gain nothing.
+    static constexpr int kPolyOf = D == 64 ? 8 : 0;
     static constexpr int kSoftWarps = 4 * kSplit, kFeedWarp = kSoftWarps, kThreads = 32 * (kSoftWarps + 1);
     static constexpr int kSide = 256 + 64 + 2 * kRows * 4;  // barriers and work, votes, the half rows' exchange
     static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + kSide;
@@ -203,15 +206,36 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// 2^x of two values on the FMA pipe, to 2^-23: with n the integer next to x (read from the low bits of
+// x + 1.5 * 2^23) and f = x - n in [-1/2, 1/2], 2^f by a polynomial of degree 5 fitted to the least relative error,
+// and n added to its exponent.  Below -127 the result is a zero or the smallest subnormal; NaN gives no finite 16-bit value.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+    const uint64_t v = pair(x.x, x.y), big = pair(12582912.0f, 12582912.0f);
+    const uint64_t t = add2(v, big);
+    const uint64_t f = fma2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), v);
+    uint64_t y = pair(0.001327647129073739f, 0.001327647129073739f);
+    y = fma2(y, f, pair(0.009675540961325169f, 0.009675540961325169f));
+    y = fma2(y, f, pair(0.05550713092088699f, 0.05550713092088699f));
+    y = fma2(y, f, pair(0.24022120237350464f, 0.24022120237350464f));
+    y = fma2(y, f, pair(0.6931469440460205f, 0.6931469440460205f));
+    y = fma2(y, f, pair(1.0000001192092896f, 1.0000001192092896f));
+    const float2 n = unpair(t), p = unpair(y);
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+}
+
 // One warp finds the sequence and tile of CTA x: sequences in order, each one's last (longest) tile first.
 __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w) {
     const int lane = threadIdx.x % 32;
     int before = 0;
     for (int s0 = 0; s0 < p.seqs; s0 += 32) {
         const int s = s0 + lane;
-        int a = 0, b = 0, tiles = 0;
+        int a = 0, b = 0, k0 = 0, k1 = 0, tiles = 0;
         if (s < p.seqs) {
             a = p.cu_q[s], b = min(p.cu_q[s + 1], p.q_tokens);
+            k0 = max(p.cu_k[s], 0), k1 = min(p.cu_k[s + 1], p.k_tokens);
             if (a >= 0 && a < b) tiles = (b - a - 1) / p.tile_tokens + 1;
         }
         int upto = tiles;
@@ -223,7 +247,6 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w
         const bool mine = tiles > 0 && x >= before + upto - tiles && x < before + upto;
         if (mine) {
             const int tile = before + upto - 1 - x;  // the last one first
-            const int k0 = max(p.cu_k[s], 0), k1 = min(p.cu_k[s + 1], p.k_tokens);
             const int klen = max(k1 - k0, 0);
             w->tok0 = a + tile * p.tile_tokens;
             w->tokens = min(p.tile_tokens, b - w->tok0);
@@ -298,22 +321,25 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int kvh = blockIdx.x % p.kv_heads;
+    // the work is found while the TMEM columns, the barriers and the tensor maps are made ready
     if (warp == 0) {
         const bool f = find_work(p, blockIdx.x / p.kv_heads, work);
         if (lane == 0) work->found = f;
-    }
-    if (threadIdx.x == 32) {
-        mbar_init(q_full, 1);
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(k_full + i, 1), mbar_init(v_full + i, 1);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            mbar_init(q_full, 1);
+            for (int i = 0; i < kStages; ++i) mbar_init(k_full + i, 1), mbar_init(v_full + i, 1);
+            mbar_init(s_full, 1), mbar_init(o_done, 1);
+            mbar_init(s_free, kSoftWarps), mbar_init(p_full, kSoftWarps);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        mbar_init(s_full, 1), mbar_init(o_done, 1);
-        mbar_init(s_free, kSoftWarps), mbar_init(p_full, kSoftWarps);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    if (!work->found) return;
-    if (warp == kFeedWarp) {
+    } else if (warp == kFeedWarp) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_q) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
+        }
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "n"(C::kTmemCols)
                      : "memory");
@@ -327,6 +353,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot, tmem_p = C::kTmemP ? tmem_slot[1] : tmem + C::kP;
+    auto leave = [&]() {
+        if (warp != kFeedWarp) return;
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kTmemCols));
+        if (C::kTmemP)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_p),
+                         "n"(C::kTmemP ? C::kTmemP : 32));
+    };
+    if (!work->found) {
+        leave();
+        return;
+    }
     const int tok0 = work->tok0, at0 = work->at0, lo = work->lo, hi = work->hi, k0 = work->k0;
     const int tiles = hi > lo ? (hi - lo - 1) / N + 1 : 0;
     // columns of the last tile that hold a visible key, in whole MMA steps
@@ -484,16 +522,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
                 if (c >= cols) continue;
                 uint32_t u[16];
 #pragma unroll
-                for (int i = c; i < c + 32; i += 2) {
-                    const float2 x = unpair(fma2(pair(s[i], s[i + 1]), scale2, off2));
-                    s[i] = x.x, s[i + 1] = x.y;
-                }
-#pragma unroll
-                for (int i = c; i < c + 32; ++i) s[i] = ex2(s[i]);
-#pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    sums[i % 2] = add2(sums[i % 2], pair(s[c + 2 * i], s[c + 2 * i + 1]));
-                    u[i] = pack2<TYPE>(s[c + 2 * i], s[c + 2 * i + 1]);
+                    const float2 x = unpair(fma2(pair(s[c + 2 * i], s[c + 2 * i + 1]), scale2, off2));
+                    const float2 e = C::kPolyOf && i % (C::kPolyOf ? C::kPolyOf : 1) == C::kPolyOf - 1 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+                    sums[i % 2] = add2(sums[i % 2], pair(e.x, e.y));
+                    u[i] = pack2<TYPE>(e.x, e.y);
                 }
                 if (!waited) {
                     ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
@@ -521,7 +554,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
         const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
         if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - off);
-        const float by = !ok ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+        // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
+        const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
         char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + half * (D / SPLIT) * 2;
         float worst = 0.0f;  // 0, or NaN
 #pragma unroll
@@ -557,13 +591,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kFeedWarp) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kTmemCols));
-        if (C::kTmemP)
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_p),
-                         "n"(C::kTmemP ? C::kTmemP : 32));
-    }
+    leave();
 }
 
 // [tokens][heads][D] rows as a 3-D map with boxes of 64 elements x heads x tokens.
