@@ -10,8 +10,16 @@
 // in 128-byte swizzled rows; S = Q K^T goes to TMEM; four warps (a thread a row) read it back, keep the
 // row's maximum and sum, and write the weights, rounded to the inputs' type, to TMEM, where they are
 // the A operand of O += P V.  V is staged as it lies in memory ([keys][d], the MN-major B operand).  S is read into
-// registers at once, so the next tile's Q K^T runs under this tile's exponentials; and two CTAs share an
-// SM (256 TMEM columns each), so one's products run under the other's softmax.
+// registers at once, so the next tile's Q K^T runs under this tile's exponentials; and three CTAs share an
+// SM (two of 128-wide heads: TMEM and shared memory allow no more), so that one's exponentials run while
+// another waits for its scores or looks for their maximum.
+//
+// What bounds it.  64-wide heads: the exponentials, one a score on a pipe of 16 a clock an SM; 128 x 64 scores take 512
+// clocks there and 256 on the tensor cores.  Measured in steady state: 600 clocks a tile; 8192 tokens of 64 heads over
+// 8: 704 us, 780 TFLOP/s, 0.47 of the measured bf16 GEMM.  Two row tiles of one persistent CTA (0.93 ms: fewer warps
+// to hide a tile's chain of waits), two threads a row (0.85 ms: the pair has to agree on its maximum) and P in S's
+// own columns (0.80 ms: Q K^T waits for P V) were slower.  128-wide heads: the tensor cores and the operands they read
+// from shared memory; 1500 tokens behind 8000: 107 us, 680 TFLOP/s.  Windows and short prompts: a CTA's start.
 //
 // The maximum is lazy: O and the sum are rescaled only when a row's maximum has grown by more
 // than 2^8 since the last time, which float32 sums and 16-bit weights (relative precision) hold without loss.
@@ -36,6 +44,7 @@ using bs::tc_fence_after;
 using bs::tc_fence_before;
 
 constexpr int kRows = 128;
+constexpr int kSoftWarps = 4, kFeedWarp = 4, kThreads = 160;
 constexpr float kLazy = 8.0f;  // log2 growth of a row's maximum that is left in the weights
 
 struct PrefillParams {
@@ -54,13 +63,10 @@ struct Cfg {
     static constexpr int kQBytes = kRows * D * 2;
     static constexpr int kTileBytes = N * D * 2;
     static constexpr int kCtas = D == 64 ? 3 : 2;  // to an SM
-    static constexpr int kSplit = D == 64 ? 1 : 2;  // threads to a row
-    // One pair of exponentials in eight on the FMA pipe.  8192 tokens of 64 heads: 733 us with none, 704 with one
-    // in eight, 713 with one in four; 128-wide heads, whose products bound them, gain nothing.
-    static constexpr int kPolyOf = D == 64 ? 8 : 0;
-    static constexpr int kSoftWarps = 4 * kSplit, kFeedWarp = kSoftWarps, kThreads = 32 * (kSoftWarps + 1);
-    static constexpr int kSide = 256 + 64 + 2 * kRows * 4;  // barriers and work, votes, the half rows' exchange
-    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + kSide;
+    // Which of sixteen pairs of exponentials the FMA pipe computes: two.  8192 tokens of 64 heads: 733 us with
+    // none, 704 with two, 713 with four; 128-wide heads, which products bound, gain nothing.
+    static __device__ constexpr bool poly(int i) { return D == 64 && i % 8 == 7; }
+    static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + 256;
     // TMEM columns: S and O in one allocation (powers of two), P in another where three CTAs share the SM
     static constexpr int kTmemCols = D == 64 ? 128 : 256, kTmemP = D == 64 ? 32 : 0;
     static constexpr int kS = 0, kO = N, kP = D == 64 ? 0 : N + D;
@@ -149,32 +155,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-// C (32 or 64) columns of this warp's lanes, waited for in the same statement.
-template <int C>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[C]) {
-    if constexpr (C == 32) {
-        bs::tmem_ld32(taddr, v);
-    } else {
-        static_assert(C == 64, "32 or 64 columns");
-        uint32_t r[64];
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,"
-            "%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
-            "tcgen05.wait::ld.sync.aligned;"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-              "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-              "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-              "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-              "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-              "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-            : "r"(taddr)
-            : "memory");
+// 64 columns of this warp's lanes, waited for in the same statement.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+    uint32_t r[64];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,"
+        "%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr)
+        : "memory");
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
-    }
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -303,11 +303,11 @@ __device__ __forceinline__ void row_again(const PrefillParams &p, int tok, int h
 }
 
 template <int D, int TYPE>
-__global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
+__global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
     prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
     using C = Cfg<D>;
-    constexpr int N = C::N, HALVES = C::kHalves, kStages = C::kStages, kFeedWarp = C::kFeedWarp, kSoftWarps = C::kSoftWarps;
+    constexpr int N = C::N, HALVES = C::kHalves, kStages = C::kStages;
     extern __shared__ __align__(1024) uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *q_s = sm, *k_s = q_s + C::kQBytes, *v_s = k_s + kStages * C::kTileBytes;
@@ -316,8 +316,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
     uint64_t *s_free = s_full + 1, *p_full = s_free + 1, *o_done = p_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_done + 1);
     Work *work = reinterpret_cast<Work *>(tmem_slot + 2);
-    int *votes = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + 256);  // [2][kSoftWarps]
-    float *swap = reinterpret_cast<float *>(votes + 2 * kSoftWarps);                // [2][kRows]
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int kvh = blockIdx.x % p.kv_heads;
@@ -445,86 +443,63 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
             weigh(j - 1);
         }
     } else {
-        // Row r is token r / group of the tile, query head r % group of the kv head.  Where two threads share a
-        // row, each takes half of a tile's keys and they agree on the maximum through their two warps' votes.
-        constexpr int SPLIT = C::kSplit, H = N / SPLIT;
-        const int r = threadIdx.x % kRows, half = SPLIT == 2 ? threadIdx.x / kRows : 0, tok = r / p.group;
-        const int head = kvh * p.group + r % p.group, at = at0 + tok;
-        const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-        auto meet = [&]() {
-            if constexpr (SPLIT == 2) asm volatile("bar.sync %0, 64;" ::"r"(warp % 4 + 1) : "memory");
-        };
+        // a thread's row: token r / group of the tile, query head r % group of the kv head
+        const int r = threadIdx.x, tok = r / p.group, head = kvh * p.group + r % p.group, at = at0 + tok;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;  // after a wait that gave up the warps go on to the end together, on what is there
+        bool ok = true;  // after a wait that gave up the warp goes on to the end on what is there, and writes NaN
         for (int j = 0; j < tiles; ++j) {
             ok &= wait_warp(s_full, (uint32_t)j & 1u, work);
             tc_fence_after();
-            const int base = lo + j * N + half * H, cols = (j + 1 == tiles ? last_cols : N) - half * H;
-            float s[H];
-            tmem_ld<H>(tmem + lanes + C::kS + half * H, s);  // columns behind the tile's last are masked
+            const int key = lo + j * N, cols = j + 1 == tiles ? last_cols : N;
+            float s[N];
+            tmem_ld64(tmem + lanes + C::kS, s);  // columns behind the tile's last are masked
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free);
-            if (base + H - 1 > at0 || (p.window > 0 && base <= hi - 1 - p.window)) {
-                const int last = at - base, first = p.window > 0 ? at - p.window + 1 - base : 0;
+            if (key + N - 1 > at0 || (p.window > 0 && key <= hi - 1 - p.window)) {
+                const int last = at - key, first = p.window > 0 ? at - p.window + 1 - key : 0;
 #pragma unroll
-                for (int i = 0; i < H; ++i)
+                for (int i = 0; i < N; ++i)
                     if (i > last || i < first) s[i] = -INFINITY;
             }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // chains short enough to overlap
 #pragma unroll
-            for (int i = 0; i < H; i += 8)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) tops[e] = fmaxf(fmaxf(tops[e], s[i + 2 * e]), s[i + 2 * e + 1]);
-            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            const bool grown = __any_sync(0xffffffffu, (top - m) * p.scale_log2 > kLazy);
-            bool any = grown;
-            if constexpr (SPLIT == 2) {
-                int *vote = votes + (j & 1) * kSoftWarps;
-                if (lane == 0) vote[warp] = grown;
-                meet();
-                any = vote[warp] | vote[warp ^ 4];
-            }
+            for (int i = 0; i < N; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             bool waited = j == 0;  // P and O are free once the products of the tile before are done
-            if (any) {
-                if constexpr (SPLIT == 2) {
-                    swap[threadIdx.x] = top;
-                    meet();
-                    top = fmaxf(top, swap[threadIdx.x ^ kRows]);
-                }
+            if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > kLazy)) {
                 const float mm = fmaxf(m, top);
                 if (j > 0) {
-                    if (!waited) {
-                        ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
-                        tc_fence_after();
-                    }
+                    ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
                     waited = true;
+                    tc_fence_after();
                     const float keep = mm == -INFINITY ? 1.0f : ex2((m - mm) * p.scale_log2);
                     l *= keep;
 #pragma unroll
-                    for (int c = 0; c < D / SPLIT; c += 16) {
+                    for (int c = 0; c < D; c += 16) {
                         float o[16];
-                        bs::tmem_ld16(tmem + lanes + C::kO + half * (D / SPLIT) + c, o);
+                        bs::tmem_ld16(tmem + lanes + C::kO + c, o);
                         uint32_t u[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * keep);
-                        tmem_st16(tmem + lanes + C::kO + half * (D / SPLIT) + c, u);
+                        tmem_st16(tmem + lanes + C::kO + c, u);
                     }
                 }
                 m = mm;
-                meet();  // the exchange is read before the next one
             }
             const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
-            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), off2 = pair(-off, -off);
+            const uint64_t off2 = pair(-off, -off);
             uint64_t sums[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < H; c += 32) {
+            for (int c = 0; c < N; c += 32) {
                 if (c >= cols) continue;
                 uint32_t u[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float2 x = unpair(fma2(pair(s[c + 2 * i], s[c + 2 * i + 1]), scale2, off2));
-                    const float2 e = C::kPolyOf && i % (C::kPolyOf ? C::kPolyOf : 1) == C::kPolyOf - 1 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+                    const float2 e = C::poly(i) ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
                     sums[i % 2] = add2(sums[i % 2], pair(e.x, e.y));
                     u[i] = pack2<TYPE>(e.x, e.y);
                 }
@@ -533,9 +508,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
                     waited = true;
                     tc_fence_after();
                 }
-                tmem_st16(tmem_p + lanes + (half * H + c) / 2, u);
+                tmem_st16(tmem_p + lanes + c / 2, u);
             }
-            if (!waited) ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
             const float2 sum = unpair(add2(sums[0], sums[1]));
             l += sum.x + sum.y;
             tmem_wait_st();
@@ -545,25 +519,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
         }
         if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
-        if constexpr (SPLIT == 2) {
-            swap[threadIdx.x] = l;
-            meet();
-            l += swap[threadIdx.x ^ kRows];
-            meet();
-        }
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
-        const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
-        if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - off);
+        if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - (m == -INFINITY ? 0.0f : m * p.scale_log2));
         // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
         const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
-        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + half * (D / SPLIT) * 2;
-        float worst = 0.0f;  // 0, or NaN
+        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
+        float worst = l * 0.0f;  // 0, or NaN
 #pragma unroll
-        for (int c = 0; c < D / SPLIT; c += 32) {
+        for (int c = 0; c < D; c += 32) {
             float o[32];
             __syncwarp();
             if (tiles > 0) {
-                bs::tmem_ld32(tmem + lanes + C::kO + half * (D / SPLIT) + c, o);
+                bs::tmem_ld32(tmem + lanes + C::kO + c, o);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0.0f;
@@ -580,13 +547,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, Cfg<D>::kCtas)
                 }
             }
         }
-        __syncwarp();
-        if constexpr (SPLIT == 2) {
-            swap[threadIdx.x] = worst;
-            meet();
-            worst += swap[threadIdx.x ^ kRows];
-        }
-        if (half == 0 && mine && ok && (worst != 0.0f || !isfinite(l)))
+        if (mine && ok && worst != 0.0f)
             row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
     }
     tc_fence_before();
@@ -620,7 +581,7 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_release);
     }
-    kernel<<<grid, Cfg<D>::kThreads, Cfg<D>::kSmem, st>>>(q, k, v, p);
+    kernel<<<grid, kThreads, Cfg<D>::kSmem, st>>>(q, k, v, p);
     return cudaGetLastError();
 }
 
