@@ -98,11 +98,20 @@ def _stream(stream, device: int):
     return stream.cuda_stream, stream
 
 
-def _empty(shape, dtype, device, stream):
+def _like(t, dtype, stream):
+    """A new contiguous tensor of t's shape (empty_like: half the host time of empty)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _empty(like, shape, dtype, stream):
+    """A new tensor on like's device."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _attn(scale, window: int, sinks, heads: int, device: int) -> bytes:
@@ -212,7 +221,7 @@ class KVCache:
         if q is not None:
             cq = _rows(q, "q", n, d, dev)
             if q_out is None:
-                q_out = _empty(q.shape, q_type or q.dtype, self.device, st)
+                q_out = _like(q, q_type, st)
             else:
                 if q_type is not None and q_out.dtype != q_type:
                     _invalid(f"q_out is {q_out.dtype}, q_type {q_type}")
@@ -245,11 +254,11 @@ class KVCache:
             dtype = torch.bfloat16 if self.k_scale is not None else self.k.dtype
         shape = (total, self.kv_heads, d)
         if k_out is None:
-            k_out = _empty(shape, dtype, self.device, st)
+            k_out = _empty(self.k, shape, dtype, st)
         else:
             _written(k_out, "k_out")
         if v_out is None:
-            v_out = _empty(shape, dtype, self.device, st)
+            v_out = _empty(self.k, shape, dtype, st)
         else:
             _written(v_out, "v_out")
         rc = self._lib.amoe_kv_read(
@@ -270,7 +279,7 @@ class KVCache:
         cq = _rows(q, "q", count, d, dev)
         heads = q.shape[1]
         if out is None:
-            out = _empty((count, heads, d), q.dtype, self.device, st)
+            out = _like(q, None, st)
         else:
             _written(out, "out")
         shape = (count, page_table.shape[1], heads, window, max_len)
@@ -281,7 +290,7 @@ class KVCache:
             if len(self._workspace) > 1000:
                 self._workspace.clear()
             self._workspace[shape] = size
-        work = _empty((size,), torch.uint8, self.device, st) if size else None
+        work = _empty(self.k, size, torch.uint8, st) if size else None
         rc = self._lib.amoe_attn_decode(
             self._at, seqs, _attn(scale, window, sinks, heads, dev), cq, _rows(out, "out", count, d, dev),
             _ints(kv_len, "kv_len", count, dev), max_len, None if work is None else work.data_ptr(), size, raw)
@@ -317,7 +326,7 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: float | None = None, window: int = 
     n, heads, d = q.shape
     m = k.shape[0]
     if out is None:
-        out = _empty((n, heads, d), q.dtype, q.device, st)
+        out = _like(q, None, st)
     else:
         _written(out, "out")
     rc = lib.amoe_attn_prefill(
