@@ -41,9 +41,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr float kLazy = 8.0f;  // log2 growth of a head's maximum that is left in the weights
 constexpr int kCluster = 8;
 constexpr int kMaxWide = 256;  // CTAs that the join kernel takes: one for each of its threads
-constexpr int kRingBytes = 16 * 1024;
 
 struct DecodeParams {
     CacheDev c;
@@ -108,13 +108,27 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// An 8 x 8 matrix of 16-bit elements, two of a row to a lane, transposed across the warp.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 __device__ __forceinline__ float quad_max(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
     return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
-__device__ __forceinline__ float quad_sum(float x) {
-    x += __shfl_xor_sync(0xffffffffu, x, 1);
-    return x + __shfl_xor_sync(0xffffffffu, x, 2);
+// Over the eight lanes that hold the same pair of heads.
+__device__ __forceinline__ float keys_max(float x) {
+#pragma unroll
+    for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
+    return x;
+}
+__device__ __forceinline__ float keys_sum(float x) {
+#pragma unroll
+    for (int i = 4; i < 32; i <<= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+    return x;
 }
 
 // Sizes of one instantiation.  TYPE is the products' type: the cache's, or F16 for E4M3.
@@ -178,11 +192,11 @@ __device__ __forceinline__ void finish(const DecodeParams &p, int seq, int h, in
     store_row(p, seq, h, i % (D / 4), a, sum, top, y);
 }
 
-template <int D, int CACHE, bool HI, bool WIDE>
+template <int D, int CACHE, int NB, bool WIDE>
 __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_kernel(const __grid_constant__ DecodeParams p) {
     using T = Tile<D, CACHE>;
     constexpr int TYPE = T::kType, KEYS = T::kKeys, ROW = T::kRow, STAGES = T::kStages;
-    constexpr int CPR = ROW / 16, NT = KEYS / 8, ROWS = HI ? 2 : 1;
+    constexpr int CPR = ROW / 16, MT = KEYS / 16;
     extern __shared__ __align__(128) char smem[];
     namespace cg = cooperative_groups;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
@@ -205,25 +219,23 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_k
     const int ntile = end > from ? (end - base - 1) / KEYS + 1 : 0;
     const int t0 = (int)((int64_t)ntile * rank / split) + warp, t1 = (int)((int64_t)ntile * (rank + 1) / split);
 
-    // the queries: rows g and g + 8 of the group, as the products' A operand
-    uint32_t qa[D / 16][4];
-    float qscale[2] = {p.scale_log2, p.scale_log2};
+    // The queries of NB blocks of eight heads as the scores' B operand: lane's head g of a block.  qs: the factors of the
+    // heads 2c and 2c + 1 whose scores the lane gets.
+    uint32_t qb[NB][D / 16][2];
+    float qs[NB][2];
 #pragma unroll
-    for (int hi = 0; hi < 2; ++hi) {
-        const int r = row0 + g + 8 * hi;
-        const bool live = r < p.group && (HI || hi == 0);
+    for (int nb = 0; nb < NB; ++nb) {
+        const int r = row0 + g + 8 * nb;
+        const bool live = r < p.group;
         const char *src = p.q.p + seq * p.q.ts + (int64_t)(kvh * p.group + (live ? r : 0)) * p.q.hs;
         auto pair = [&](int d) -> uint32_t { return live ? *reinterpret_cast<const uint32_t *>(src + d * 2) : 0u; };
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-            if constexpr (T::kFp8) {
-                // a thread's 16-byte chunk of a key holds four steps' operands of its column pair
-                const int d = (c * (D / 64) + ks / 4) * 16 + ks % 4 * 4;
-                qa[ks][hi] = pair(d), qa[ks][hi + 2] = pair(d + 2);
-            } else {
-                qa[ks][hi] = pair(ks * 16 + 2 * c), qa[ks][hi + 2] = pair(ks * 16 + 2 * c + 8);
-            }
+            // E4M3: a thread's 16-byte chunk of a key holds four steps' operands of its column pair
+            const int d = T::kFp8 ? (c * (D / 64) + ks / 4) * 16 + ks % 4 * 4 : ks * 16 + 2 * c;
+            qb[nb][ks][0] = pair(d), qb[nb][ks][1] = pair(T::kFp8 ? d + 2 : d + 8);
         }
+        float factor = p.scale_log2;
         if (T::kFp8 && p.q_type == AMOE_GGUF_BF16) {
             // bf16 queries as f16: the row's largest value brought to [1, 2) by a power of two, which
             // the score gets back; what f16 then loses is below 2^-25 of that value
@@ -231,22 +243,24 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_k
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-                for (int i = hi; i < 4; i += 2) {
-                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qa[ks][i]));
+                for (int i = 0; i < 2; ++i) {
+                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qb[nb][ks][i]));
                     big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
                 }
             big = quad_max(big);
             const int e = big > 0.0f ? min(max((int)(__float_as_uint(big) >> 23) - 127, -126), 126) : 0;
             const float by = __uint_as_float((uint32_t)(127 - e) << 23);
-            qscale[hi] *= __uint_as_float((uint32_t)(127 + e) << 23);
+            factor *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-                for (int i = hi; i < 4; i += 2) {
-                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qa[ks][i]));
-                    qa[ks][i] = pack2<AMOE_GGUF_F16>(f.x * by, f.y * by);
+                for (int i = 0; i < 2; ++i) {
+                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qb[nb][ks][i]));
+                    qb[nb][ks][i] = pack2<AMOE_GGUF_F16>(f.x * by, f.y * by);
                 }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qs[nb][i] = __shfl_sync(0xffffffffu, factor, (2 * c + i) * 4);
     }
 
     // A tile lies in one page where pages hold whole tiles; otherwise each lane looks its key's page up.
@@ -323,8 +337,12 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_k
         if (lane == 0) masks[stage] = live;
     };
 
-    float o[D / 8][4] = {};
-    float m[2] = {-INFINITY, -INFINITY}, n[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    // o: rows are elements, columns heads; m, n, l: of the lane's two heads of each block, l over its own keys
+    float o[D / 16][NB][4] = {}, m[NB][2], n[NB][2], l[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m[nb][i] = n[nb][i] = -INFINITY, l[nb][i] = 0.0f;
     {
         int pages[STAGES - 1];
 #pragma unroll
@@ -360,126 +378,142 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_k
             __syncwarp();
         }
 
-        // scores
-        float s[NT][4];
+        // scores: rows are keys, columns heads
+        float sc[MT][NB][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+        for (int t16 = 0; t16 < MT; ++t16) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) sc[t16][nb][0] = sc[t16][nb][1] = sc[t16][nb][2] = sc[t16][nb][3] = 0.0f;
             if constexpr (T::kFp8) {
 #pragma unroll
                 for (int seg = 0; seg < D / 64; ++seg) {
-                    uint32_t w[4];
-                    const uint32_t a = kt + chunk_at<ROW>(j * 8 + g, c * (D / 64) + seg);
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                 : "r"(a)
-                                 : "memory");
+                    uint32_t w[2][4];
+#pragma unroll
+                    for (int hi = 0; hi < 2; ++hi) {
+                        const uint32_t a = kt + chunk_at<ROW>(t16 * 16 + hi * 8 + g, c * (D / 64) + seg);
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(w[hi][0]), "=r"(w[hi][1]), "=r"(w[hi][2]), "=r"(w[hi][3])
+                                     : "r"(a)
+                                     : "memory");
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        uint32_t b0, b1;
-                        e4m3x4_to_f16x2(w[i], b0, b1);
-                        mma16<TYPE>(s[j], qa[seg * 4 + i], b0, b1);
+                        uint32_t a[4];
+                        e4m3x4_to_f16x2(w[0][i], a[0], a[2]);
+                        e4m3x4_to_f16x2(w[1][i], a[1], a[3]);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            mma16<TYPE>(sc[t16][nb], a, qb[nb][seg * 4 + i][0], qb[nb][seg * 4 + i][1]);
                     }
                 }
             } else {
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ks += 2) {
-                    uint32_t b[4];
-                    ldm4(b, kt + chunk_at<ROW>(j * 8 + lane % 8, ks * 2 + lane / 8));
-                    mma16<TYPE>(s[j], qa[ks], b[0], b[1]);
-                    mma16<TYPE>(s[j], qa[ks + 1], b[2], b[3]);
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    uint32_t a[4];
+                    ldm4(a, kt + chunk_at<ROW>(t16 * 16 + lane % 16, ks * 2 + lane / 16));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) mma16<TYPE>(sc[t16][nb], a, qb[nb][ks][0], qb[nb][ks][1]);
                 }
             }
         }
         // to log2; E4M3: with the keys' scales, the values' exponents beside
-        float ev[NT][2];
+        float ev[MT][2];
+        bool grown = false;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            float by[2] = {1.0f, 1.0f};
-            if constexpr (T::kFp8) {
-                const float4 x = reinterpret_cast<const float4 *>(side + stage * 64)[j * 4 + c];
-                by[0] = x.x, ev[j][0] = x.y, by[1] = x.z, ev[j][1] = x.w;
-            }
+        for (int t16 = 0; t16 < MT; ++t16)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int hi = 0; hi < 2; ++hi) {
+                float by = 1.0f;
+                ev[t16][hi] = 0.0f;
+                if constexpr (T::kFp8) {
+                    const float2 x = reinterpret_cast<const float2 *>(side + stage * 64)[t16 * 16 + hi * 8 + g];
+                    by = x.x, ev[t16][hi] = x.y;
+                }
+                const bool on = mask >> (t16 * 16 + hi * 8 + g) & 1u;
 #pragma unroll
-                for (int hi = 0; hi < ROWS; ++hi) s[j][2 * hi + i] *= T::kFp8 ? by[i] * qscale[hi] : qscale[hi];
-        }
-        if (mask != FULL) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int hi = 0; hi < ROWS; ++hi)
-                        if (!(mask >> (j * 8 + 2 * c + i) & 1u)) s[j][2 * hi + i] = -INFINITY;
-        }
-        // the running maximum, the weights and their sum
-        uint32_t pa[NT / 2][4];
-#pragma unroll
-        for (int hi = 0; hi < 2; ++hi) {
-            if (hi >= ROWS) {
-#pragma unroll
-                for (int j = 0; j < NT / 2; ++j) pa[j][1] = pa[j][3] = 0u;
-                continue;
-            }
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) top = fmaxf(top, s[j][2 * hi + i]);
-            if constexpr (T::kFp8) {
-                const float nn = fmaxf(n[hi], quad_max(top)), z = nn == -INFINITY ? 0.0f : nn;
-                l[hi] *= ex2(n[hi] - z);
-                n[hi] = nn;
-                top = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        sum += ex2(s[j][2 * hi + i] - z);
-                        s[j][2 * hi + i] += ev[j][i];
-                        top = fmaxf(top, s[j][2 * hi + i]);
+                        float &x = sc[t16][nb][2 * hi + i];
+                        x = on ? x * (T::kFp8 ? by * qs[nb][i] : qs[nb][i]) : -INFINITY;
+                        if constexpr (T::kFp8) grown |= x - n[nb][i] > kLazy;
+                        grown |= x + ev[t16][hi] - m[nb][i] > kLazy;
                     }
             }
-            const float mm = fmaxf(m[hi], quad_max(top)), z = mm == -INFINITY ? 0.0f : mm;
-            if (__any_sync(0xffffffffu, mm != m[hi])) {
-                const float keep = ex2(m[hi] - z);
-                if constexpr (!T::kFp8) l[hi] *= keep;
+        // The maxima are lazy: they move, and what hangs on them with them, when some weight outgrew its own by 2^8.
+        if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) o[j][2 * hi] *= keep, o[j][2 * hi + 1] *= keep;
-                m[hi] = mm;
-            }
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const float a = ex2(s[j][2 * hi] - z), b = ex2(s[j][2 * hi + 1] - z);
-                if constexpr (!T::kFp8) sum += a + b;
-                pa[j / 2][hi + 2 * (j % 2)] = pack2<TYPE>(a, b);
-            }
-            l[hi] += sum;
+                for (int i = 0; i < 2; ++i) {
+                    float top = -INFINITY, ntop = -INFINITY;
+#pragma unroll
+                    for (int t16 = 0; t16 < MT; ++t16)
+#pragma unroll
+                        for (int hi = 0; hi < 2; ++hi) {
+                            top = fmaxf(top, sc[t16][nb][2 * hi + i] + ev[t16][hi]);
+                            ntop = fmaxf(ntop, sc[t16][nb][2 * hi + i]);
+                        }
+                    const float mm = fmaxf(m[nb][i], keys_max(top)), keep = ex2(m[nb][i] - (mm == -INFINITY ? 0.0f : mm));
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) o[j][nb][i] *= keep, o[j][nb][2 + i] *= keep;
+                    m[nb][i] = mm;
+                    if constexpr (T::kFp8) {
+                        const float nn = fmaxf(n[nb][i], keys_max(ntop));
+                        l[nb][i] *= ex2(n[nb][i] - (nn == -INFINITY ? 0.0f : nn));
+                        n[nb][i] = nn;
+                    } else {
+                        l[nb][i] *= keep;
+                    }
+                }
         }
-        // weights times values
+        // the weights, transposed to the B operand of the values' products
+        uint32_t pb[MT][NB][2];
 #pragma unroll
-        for (int ks = 0; ks < NT / 2; ++ks) {
-            const int r = ks * 16 + lane % 16;
+        for (int nb = 0; nb < NB; ++nb) {
+            float z[2], y[2];
 #pragma unroll
-            for (int j = 0; j < CPR; j += 2) {
-                uint32_t b[4];
-                ldm4t(b, vt + chunk_at<ROW>(r, j + lane / 16));
-                if constexpr (T::kFp8) {
-                    // a register holds two keys' codes of elements 2g and 2g + 1 of the chunk: element pairs
-                    // become key pairs, and even and odd elements two tiles of eight columns
+            for (int i = 0; i < 2; ++i) {
+                z[i] = m[nb][i] == -INFINITY ? 0.0f : m[nb][i];
+                y[i] = n[nb][i] == -INFINITY ? 0.0f : n[nb][i];
+            }
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t even0, odd0, even1, odd1;
-                        e4m3x4_to_f16x2(__byte_perm(b[2 * x], 0, 0x3120), even0, odd0);
-                        e4m3x4_to_f16x2(__byte_perm(b[2 * x + 1], 0, 0x3120), even1, odd1);
-                        mma16<TYPE>(o[2 * (j + x)], pa[ks], even0, even1);
-                        mma16<TYPE>(o[2 * (j + x) + 1], pa[ks], odd0, odd1);
+            for (int t16 = 0; t16 < MT; ++t16)
+#pragma unroll
+                for (int hi = 0; hi < 2; ++hi) {
+                    float w[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float x = sc[t16][nb][2 * hi + i];
+                        w[i] = ex2(x + ev[t16][hi] - z[i]);
+                        l[nb][i] += T::kFp8 ? ex2(x - y[i]) : w[i];
                     }
-                } else {
-                    mma16<TYPE>(o[j], pa[ks], b[0], b[1]);
-                    mma16<TYPE>(o[j + 1], pa[ks], b[2], b[3]);
+                    pb[t16][nb][hi] = transposed(pack2<TYPE>(w[0], w[1]));
+                }
+        }
+        // values times weights: rows are elements, columns heads
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+            if constexpr (T::kFp8) {
+                // a register holds two keys' codes of elements 2g and 2g + 1 of the chunk: element pairs become key pairs,
+                // even elements the upper eight rows and odd ones the lower
+                uint32_t b[4];
+                ldm4t(b, vt + chunk_at<ROW>(lane, j));
+#pragma unroll
+                for (int t16 = 0; t16 < MT; ++t16) {
+                    uint32_t a[4];
+                    e4m3x4_to_f16x2(__byte_perm(b[2 * t16], 0, 0x3120), a[0], a[1]);
+                    e4m3x4_to_f16x2(__byte_perm(b[2 * t16 + 1], 0, 0x3120), a[2], a[3]);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) mma16<TYPE>(o[j][nb], a, pb[t16][nb][0], pb[t16][nb][1]);
+                }
+            } else {
+#pragma unroll
+                for (int t16 = 0; t16 < MT; ++t16) {
+                    uint32_t a[4];
+                    ldm4t(a, vt + chunk_at<ROW>(t16 * 16 + lane % 8 + lane / 16 * 8, j * 2 + lane / 8 % 2));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) mma16<TYPE>(o[j][nb], a, pb[t16][nb][0], pb[t16][nb][1]);
                 }
             }
         }
@@ -495,28 +529,26 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_k
     {
         float *mine = part + (1 + warp) * T::kPart;
 #pragma unroll
-        for (int hi = 0; hi < 2; ++hi) {
-            const float sum = quad_sum(l[hi]);
-            const int r = g + 8 * hi;
-            if (c == 0) {
-                mine[16 * D + r] = m[hi];
-                mine[16 * D + 16 + r] = T::kFp8 ? n[hi] : m[hi];
-                mine[16 * D + 32 + r] = sum;
-            }
-            if (hi >= ROWS) continue;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-                if constexpr (T::kFp8) {
-                    float *x = mine + r * D + j / 2 * 16 + 4 * c + j % 2;
-                    x[0] = o[j][2 * hi], x[2] = o[j][2 * hi + 1];
-                } else {
-                    *reinterpret_cast<float2 *>(mine + r * D + j * 8 + 2 * c) = make_float2(o[j][2 * hi], o[j][2 * hi + 1]);
+            for (int i = 0; i < 2; ++i) {
+                const float sum = keys_sum(l[nb][i]);
+                const int r = nb * 8 + 2 * c + i;
+                if (g == 0) {
+                    mine[16 * D + r] = m[nb][i];
+                    mine[16 * D + 16 + r] = T::kFp8 ? n[nb][i] : m[nb][i];
+                    mine[16 * D + 32 + r] = sum;
+                }
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    float *x = mine + r * D + j * 16;
+                    x[T::kFp8 ? 2 * g : g] = o[j][nb][i];
+                    x[T::kFp8 ? 2 * g + 1 : g + 8] = o[j][nb][2 + i];
                 }
             }
-        }
     }
     __syncthreads();
-    constexpr int LIVE = HI ? 16 : 8;  // rows of the tile that the instantiation fills
+    constexpr int LIVE = 8 * NB;  // heads of the tile that the instantiation fills
     for (int i = threadIdx.x; i < LIVE * D / 4; i += kThreads) {
         const int r = i / (D / 4);
         float top = -INFINITY;
@@ -628,10 +660,10 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
 
 constexpr int kMaxDevices = 64;
 
-template <int D, int CACHE, bool HI, bool WIDE>
+template <int D, int CACHE, int NB, bool WIDE>
 cudaError_t launch(const DecodeParams &p, int device, int units, int seqs, cudaStream_t st) {
     using T = Tile<D, CACHE>;
-    auto *kernel = decode_attn_kernel<D, CACHE, HI, WIDE>;
+    auto *kernel = decode_attn_kernel<D, CACHE, NB, WIDE>;
     static std::atomic<bool> ready[kMaxDevices];
     if (!ready[device].load(std::memory_order_acquire)) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
@@ -651,7 +683,7 @@ cudaError_t launch(const DecodeParams &p, int device, int units, int seqs, cudaS
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess || !WIDE) return e;
     cudaLaunchConfig_t join{};
-    join.gridDim = dim3(HI ? 16 : 8, units, seqs);
+    join.gridDim = dim3(8 * NB, units, seqs);
     join.blockDim = dim3(kJoinThreads);
     join.stream = st;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -701,10 +733,10 @@ Layout layout_of(int D, int cache, int64_t units, int64_t seqs, int64_t tokens) 
 template <int D, int CACHE>
 cudaError_t launch_rows(const DecodeParams &p, int device, int units, int seqs, bool wide, cudaStream_t st) {
     if (p.group > 8)
-        return wide ? launch<D, CACHE, true, true>(p, device, units, seqs, st)
-                    : launch<D, CACHE, true, false>(p, device, units, seqs, st);
-    return wide ? launch<D, CACHE, false, true>(p, device, units, seqs, st)
-                : launch<D, CACHE, false, false>(p, device, units, seqs, st);
+        return wide ? launch<D, CACHE, 2, true>(p, device, units, seqs, st)
+                    : launch<D, CACHE, 2, false>(p, device, units, seqs, st);
+    return wide ? launch<D, CACHE, 1, true>(p, device, units, seqs, st)
+                : launch<D, CACHE, 1, false>(p, device, units, seqs, st);
 }
 
 template <int D>
