@@ -2,18 +2,20 @@
 // (CausalAttentionWithConfig with one query, internal/backend/cpuref/attention.go:82-171).
 //
 // A step reads every visible key and value once and does a handful of products with each, so
-// HBM bounds it.  What the kernel does about that:
-//   - the query heads of one kv head are the rows of one tile, so keys are read once for all of
-//     them; products run on mma.sync m16n8k16 (16 rows; groups up to 8 leave the upper half
-//     empty).  CUDA cores could not keep up: 8 heads x 2 products an element at 6.5 TB/s is
-//     two thirds of the f32 rate for 16-bit caches and over it for E4M3;
+// HBM bounds it, or the instructions that get E4M3 codes to the products.  What the kernel does about that:
+//   - the query heads of one kv head share one read of its keys, as columns of mma.sync m16n8k16
+//     products whose rows are keys (scores) and elements (values): eight heads fill a block.  CUDA cores could not
+//     keep up: 8 heads x 2 products an element at 6.5 TB/s is two thirds of the f32 rate for 16-bit
+//     caches and over it for E4M3;
 //   - each warp walks its own tiles of 32 (16 for 128-wide 16-bit rows) keys through a private
-//     ring of cp.async copies, so no barrier stands in the loop; 12 to 16 warps of two or three
-//     stages keep 100 to 200 KB an SM in flight, more than latency times bandwidth needs (deeper rings
-//     with fewer warps were slower: a tile is a chain of dependent steps, and warps hide it).  Each copy
-//     carries its own length, so a masked key, or one without a page, is staged as zeros: what
-//     lies in such slots, NaN included, never reaches the products.  A tile that lies in one page
-//     is copied as one run; smaller pages have each lane look up its key;
+//     ring of two cp.async stages, so no barrier stands in the loop; 12 to 20 warps an SM keep 100 to 200 KB
+//     in flight, more than latency times bandwidth needs (deeper rings with fewer warps were slower: a
+//     tile is a chain of dependent steps, and warps hide it).  Each copy carries its own length, so a
+//     masked key, or one without a page, is staged as zeros: what lies in such slots, NaN included,
+//     never reaches the products.  A tile that lies in one page is copied as one run; smaller pages
+//     have each lane look up its key;
+//   - a head's running maximum is lazy: it moves, and the sums are rescaled, when some weight has outgrown it by
+//     2^8, which one vote a tile finds out;
 //   - the keys of one (sequence, kv head) are split over the CTAs of a cluster of up to 8, whose
 //     partial sums join through distributed shared memory: one launch.  A few long sequences
 //     need more CTAs than clusters can place (clusters of 16 left SMs idle: 59 us instead of 50 for
@@ -21,13 +23,15 @@
 //     a second kernel, whose launch overlaps the first, joins them.  No atomics: the order of addition
 //     does not depend on timing.
 //
-// Measured (B200): 131072 tokens, 8 kv heads, f16: 49.7 us, 5.4 TB/s, 0.82 of the copy bandwidth.
-// 48 sequences of 4096-8192, E4M3: 79 us, 3.8 TB/s, bound by instruction issue (conversions).
-//
 // E4M3 keys and values meet f16 operands (every code is an f16 value).  A key's scale multiplies
 // its score.  A value's scale 2^e goes into the weight: w = exp2(t + e - m), t the score in
 // log2 and m the running maximum of t + e, so the 16-bit weight keeps its precision whatever
 // the scales are; the denominator sums exp2(t - n) with a maximum n of its own.
+//
+// Measured (B200): 131072 tokens, 8 kv heads, f16: 49.2 us, 5.5 TB/s, 0.83 of the copy bandwidth.
+// 48 sequences of 4096-8192 tokens, E4M3: 70 us, 4.3 TB/s, 0.66: the ALU pipe is 44 % busy (the codes'
+// conversions) and sequences of unequal lengths leave SMs idle at the end.  E4M3 products (m16n8k32, queries
+// and weights as two E4M3 terms each) took 89 us.
 #include "attn.cuh"
 
 #include <cooperative_groups.h>
@@ -139,8 +143,8 @@ struct Tile {
     static constexpr int kRow = D * (kFp8 ? 1 : 2);             // bytes of a cache row
     static constexpr int kKeys = kRow == 256 ? 16 : 32;         // keys of a warp's tile
     static constexpr int kStage = 2 * kKeys * kRow;             // K then V
-    static constexpr int kStages = kStage == 4096 ? 3 : 2;
-    static constexpr int kCtas = kStage == 4096 ? 4 : 3;        // to an SM: what registers and shared memory allow
+    static constexpr int kStages = 2;
+    static constexpr int kCtas = kStage == 4096 ? 5 : 3;        // to an SM: what registers and shared memory allow
     static constexpr int kSide = kFp8 ? 256 : 0;                // two words of scales a key
     static constexpr int kWarpBytes = kStages * kStage + kStages * (kSide + 4);
     static constexpr int kSmem = kWarps * ((kWarpBytes + 127) / 128 * 128);
@@ -193,7 +197,7 @@ __device__ __forceinline__ void finish(const DecodeParams &p, int seq, int h, in
 }
 
 template <int D, int CACHE, int NB, bool WIDE>
-__global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas) decode_attn_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && Tile<D, CACHE>::kCtas > 3)) decode_attn_kernel(const __grid_constant__ DecodeParams p) {
     using T = Tile<D, CACHE>;
     constexpr int TYPE = T::kType, KEYS = T::kKeys, ROW = T::kRow, STAGES = T::kStages;
     constexpr int CPR = ROW / 16, MT = KEYS / 16;
@@ -706,7 +710,7 @@ struct Layout {
 Layout layout(int64_t units, int64_t seqs, int64_t tokens, int row_bytes, int part_floats, int ctas) {
     const int keys = row_bytes == 256 ? 16 : 32;
     const int64_t tiles = (tokens - 1) / keys + 1, all = units * seqs;
-    const int want = 4 * 148;
+    const int want = 6 * 148;
     Layout l{1, false, 0};
     while (l.split < kCluster && all * l.split < want && tiles > l.split * kWarps) l.split *= 2;
     if (l.split == kCluster && all * l.split < want / 2) {
