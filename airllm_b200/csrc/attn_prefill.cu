@@ -392,51 +392,51 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         bool ok = tiles > 0 && wait_warp(q_full, 0, work);
         auto scores = [&](int j) {  // S = Q K^T of tile j
             if (j >= tiles) return;
-                const int s = j % kStages;
-                ok = wait_warp(k_full + s, (uint32_t)(j / kStages) & 1u, work);
-                if (ok && j > 0) ok = wait_warp(s_free, (uint32_t)(j - 1) & 1u, work);
-                if (!ok) return;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t id = idesc<TYPE>(j + 1 == tiles ? last_cols : N, false);
-                    const uint64_t kd = k_d + s * (C::kTileBytes / 16);
+            const int s = j % kStages;
+            ok = wait_warp(k_full + s, (uint32_t)(j / kStages) & 1u, work);
+            if (ok && j > 0) ok = wait_warp(s_free, (uint32_t)(j - 1) & 1u, work);
+            if (!ok) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t id = idesc<TYPE>(j + 1 == tiles ? last_cols : N, false);
+                const uint64_t kd = k_d + s * (C::kTileBytes / 16);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        mma_ss(tmem + C::kS, q_d + i / 4 * (kRows * 8) + i % 4 * 2, kd + i / 4 * (N * 8) + i % 4 * 2, id, i > 0);
-                    mma_commit(s_full);
-                    if (j > 0 && j - 1 + kStages < tiles) load(k_s, &tm_k, k_full, j - 1 + kStages);
-                }
-                __syncwarp();
+                for (int i = 0; i < D / 16; ++i)
+                    mma_ss(tmem + C::kS, q_d + i / 4 * (kRows * 8) + i % 4 * 2, kd + i / 4 * (N * 8) + i % 4 * 2, id, i > 0);
+                mma_commit(s_full);
+                if (j > 0 && j - 1 + kStages < tiles) load(k_s, &tm_k, k_full, j - 1 + kStages);
+            }
+            __syncwarp();
         };
         auto weigh = [&](int t) {  // O += P V of tile t
             if (t < 0 || !ok) return;
-                const int s = t % kStages;
-                ok = wait_warp(v_full + s, (uint32_t)(t / kStages) & 1u, work);
-                if (!ok) return;
-                const int cols = t + 1 == tiles ? last_cols : N;
-                const int seen = hi - lo - t * N;
-                if (seen < cols) {  // no value behind the last visible key reaches the products
-                    for (int i = lane; i < (cols - seen) * 8 * HALVES; i += 32) {
-                        const int h = i / ((cols - seen) * 8), r = i / 8 % (cols - seen);
-                        *reinterpret_cast<uint4 *>(v_s + s * C::kTileBytes + h * N * 128 + (seen + r) * 128 + i % 8 * 16) =
-                            make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
+            const int s = t % kStages;
+            ok = wait_warp(v_full + s, (uint32_t)(t / kStages) & 1u, work);
+            if (!ok) return;
+            const int cols = t + 1 == tiles ? last_cols : N;
+            const int seen = hi - lo - t * N;
+            if (seen < cols) {  // no value behind the last visible key reaches the products
+                for (int i = lane; i < (cols - seen) * 8 * HALVES; i += 32) {
+                    const int h = i / ((cols - seen) * 8), r = i / 8 % (cols - seen);
+                    *reinterpret_cast<uint4 *>(v_s + s * C::kTileBytes + h * N * 128 + (seen + r) * 128 + i % 8 * 16) =
+                        make_uint4(0, 0, 0, 0);
                 }
-                ok = wait_warp(p_full, (uint32_t)t & 1u, work);
-                if (!ok) return;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t id = idesc<TYPE>(D, true);
-                    const uint64_t vd = v_d + s * (C::kTileBytes / 16);
-#pragma unroll
-                    for (int i = 0; i < N / 16; ++i)
-                        if (i * 16 < cols) mma_ts(tmem + C::kO, tmem_p + i * 8, vd + i * 128, id, t > 0 || i > 0);
-                    mma_commit(o_done);
-                    if (t > 0 && t - 1 + kStages < tiles) load(v_s, &tm_v, v_full, t - 1 + kStages);
-                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
+            }
+            ok = wait_warp(p_full, (uint32_t)t & 1u, work);
+            if (!ok) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t id = idesc<TYPE>(D, true);
+                const uint64_t vd = v_d + s * (C::kTileBytes / 16);
+#pragma unroll
+                for (int i = 0; i < N / 16; ++i)
+                    if (i * 16 < cols) mma_ts(tmem + C::kO, tmem_p + i * 8, vd + i * 128, id, t > 0 || i > 0);
+                mma_commit(o_done);
+                if (t > 0 && t - 1 + kStages < tiles) load(v_s, &tm_v, v_full, t - 1 + kStages);
+            }
+            __syncwarp();
         };
         for (int j = 0; ok && j <= tiles; ++j) {
             scores(j);
