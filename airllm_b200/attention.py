@@ -72,6 +72,8 @@ def _rows(t, name: str, tokens: int, head_dim: int, device: int) -> bytes:
 
 def _written(t, name: str):
     """Rows that a call writes must not share memory with one another."""
+    if t.dim() != 3:
+        _invalid(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
     n, h, d = t.shape
     st, sh, _ = t.stride()
     if (n > 1 and st < d) or (h > 1 and sh < d) or (n > 1 and h > 1 and min(st, sh) * ((h if sh <= st else n) - 1) + d
@@ -300,6 +302,7 @@ class KVCache:
 
     def check(self):
         """Waits for the device and raises if a call met a wrong page id or length since the last check."""
+        torch.cuda.synchronize(self.device)  # calls on every stream
         bits = int(self.status.item())
         if not bits:
             return

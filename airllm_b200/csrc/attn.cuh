@@ -222,7 +222,7 @@ inline int check_group(int q_heads, int kv_heads) {
 inline int check_attn(const amoe_attn *a) {
     if (!a) return reject("attn must not be NULL");
     if (a->window < 0) return reject("sliding window must be non-negative");
-    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return reject("scale must be finite and non-negative");
+    if (!(a->scale >= 0.0f) || std::isinf(a->scale * kLog2e)) return reject("scale must be finite and non-negative");
     return AMOE_OK;
 }
 

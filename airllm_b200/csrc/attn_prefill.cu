@@ -262,6 +262,12 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w
     return false;
 }
 
+// A sink's share of the denominator beside the maximum z (in log2).  It may pass float32's range, and the row is then 0;
+// a sink of +inf leaves inf / inf.
+__device__ __forceinline__ float sink_weight(float sink, float z) {
+    return sink == INFINITY ? NAN : ex2(sink * kLog2e - z);
+}
+
 // A row again, key by visible key: for results that are not finite.  Its arrays stay in local memory (no loop is
 // unrolled), so that the path costs the kernel no registers.
 template <int D, int TYPE>
@@ -293,7 +299,7 @@ __device__ __forceinline__ void row_again(const PrefillParams &p, int tok, int h
         }
     }
     const float z = m == -INFINITY ? 0.0f : m;
-    if (p.sinks) l += exp2f(p.sinks[head] * kLog2e - z);
+    if (p.sinks) l += sink_weight(p.sinks[head], z);
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
     for (int d = 0; d < D; d += 8) {
@@ -520,11 +526,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
-        if (p.sinks && mine) l += ex2(p.sinks[head] * kLog2e - (m == -INFINITY ? 0.0f : m * p.scale_log2));
+        if (p.sinks && mine) l += sink_weight(p.sinks[head], m == -INFINITY ? 0.0f : m * p.scale_log2);
         // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
         const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
         char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
-        float worst = l * 0.0f;  // 0, or NaN
+        float worst = isnan(l) ? l : 0.0f;  // 0, or NaN
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
             float o[32];
@@ -570,6 +576,7 @@ bool encode_rows(CUtensorMap *tm, const amoe_rows *r, int D, int tokens, int box
 }
 
 constexpr int kMaxDevices = 64;
+constexpr int kMaxTokens = 1 << 30;  // row indexes and positions stay far inside 32 bits
 
 template <int D, int TYPE>
 cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PrefillParams &p, int device,
@@ -599,6 +606,7 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     if (int rc = check_attn(attn)) return rc;
     if (int rc = check_head_dim(head_dim)) return rc;
     if (q_tokens < 0 || k_tokens < 0) return reject("q_tokens and k_tokens must not be negative");
+    if (q_tokens > kMaxTokens || k_tokens > kMaxTokens) return reject("more than 2^30 rows in one prefill call");
     if (int rc = check_rows(q, "q", head_dim, 0, q_tokens, -1)) return rc;
     if (q->type != AMOE_GGUF_F16 && q->type != AMOE_GGUF_BF16) return reject("prefill takes F16 or BF16 rows");
     if (int rc = check_rows(k, "k", head_dim, 0, k_tokens, q->type)) return rc;
@@ -614,7 +622,8 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     p.cu_q = cu_q, p.cu_k = cu_k;
     p.sinks = attn->sinks;
     p.scale_log2 = attn_scale(attn, head_dim) * kLog2e;
-    p.window = attn->window, p.q_tokens = q_tokens, p.k_tokens = k_tokens, p.seqs = seqs;
+    // a window as long as the keys hides none
+    p.window = attn->window < k_tokens ? attn->window : 0, p.q_tokens = q_tokens, p.k_tokens = k_tokens, p.seqs = seqs;
     p.group = q->heads / k->heads;
     p.tile_tokens = kRows / p.group;
     p.kv_heads = k->heads;

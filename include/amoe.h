@@ -397,7 +397,8 @@ AMOE_API int amoe_kv_read(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, 
 /* Scores are scale * q.k (scale 0: 1 / sqrt(head_dim)); window > 0: a query sees the last
  * `window` keys up to its own position only; sinks [q heads] (device, nullable): a learned
  * logit for each head that joins the softmax's denominator (attention.go:82-171).  A query
- * that sees no key gives a row of zeros. */
+ * that sees no key gives a row of zeros; keys and values that a query does not see do not
+ * reach its row, NaN and infinities included. */
 typedef struct amoe_attn {
     float scale;
     int32_t window;
@@ -409,7 +410,10 @@ typedef struct amoe_attn {
  * sequence s, whose queries are the last of its keys' positions; each sees the keys up to
  * its own.  q, k, v and out have one type, F16 or BF16; products accumulate in float32 and
  * the softmax's maximum and sum are float32, its weights rounded to that type.  q_tokens and
- * k_tokens are the rows given; rows of out from cu_q[seqs] on are left as they are. */
+ * k_tokens (at most 2^30) are the rows given; rows of out from cu_q[seqs] on are left as they
+ * are, and starts that decrease or pass the rows given are clamped to them.  Strides must be
+ * such as a CUDA tensor map takes.  A wait inside the kernel that gives up after about a
+ * second leaves NaN rows. */
 AMOE_API int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, const amoe_rows *q,
                                const amoe_rows *k, const amoe_rows *v, const amoe_rows *out, int32_t q_tokens,
                                int32_t k_tokens, const int32_t *cu_q, const int32_t *cu_k, int32_t seqs,

@@ -593,3 +593,144 @@ def test_python_refusals(cuda_device):
     assert attention.prefill(none, none, none, i32([0, 0]).cuda()).shape == (0, 2, 64)
     assert cache.read(table, i32([0, 0]).cuda(), 0)[0].shape == (0, 2, 64)
     cache.check()
+
+
+# ---- layouts, counts and values at the edges -----------------------------------------------------
+def test_many_sequences(cuda_device):
+    """More sequences than a warp looks at at once, empty ones among them, for each operator."""
+    g = gen(51)
+    n, heads, kv, d, page = 150, 8, 2, 64, 8
+    new = [int(x) for x in torch.randint(0, 4, (n,), generator=g)]
+    past = [int(x) for x in torch.randint(0, 20, (n,), generator=g)]
+    lens = [a + b for a, b in zip(new, past)]
+    table, pool = table_for(g, lens, page)
+    pages = filled(g, pool, kv, page, d, F16)
+    total = sum(new)
+    x = randn(g, total, heads + 2 * kv, d, dtype=F16)
+    dev, cache = x.cuda(), on_gpu(pages)
+    cache.append(dev[:, heads:heads + kv], dev[:, heads + kv:], table.cuda(), i32(past).cuda(), starts(new).cuda())
+    k, v = cache.read(table.cuda(), starts(lens).cuda(), sum(lens))
+    out = attention.prefill(dev[:, :heads], k, v, starts(new).cuda(), starts(lens).cuda())
+    one = torch.randn(n, heads, d, generator=g).half()
+    dec = cache.decode(one.cuda(), table.cuda(), i32(lens).cuda())
+    cache.check()
+    a = b = 0
+    for i in range(n):
+        held = [R.rows_of(c, s, table[i], 0, past[i]).half() for c, s in pages]
+        kk = torch.cat((held[0], x[a:a + new[i], heads:heads + kv]))
+        vv = torch.cat((held[1], x[a:a + new[i], heads + kv:]))
+        assert torch.equal(k[b:b + lens[i]].cpu(), kk) and torch.equal(v[b:b + lens[i]].cpu(), vv)
+        if new[i]:
+            R.close(out[a:a + new[i]], *R.attention(x[a:a + new[i], :heads], kk, vv))
+        if lens[i]:
+            R.close(dec[i:i + 1], *R.attention(one[i:i + 1], kk, vv))
+        else:
+            assert (dec[i] == 0).all()
+        a, b = a + new[i], b + lens[i]
+
+
+def test_prefill_layouts(cuda_device):
+    """Heads outermost, wide gaps between rows, one head of a shared buffer, and a key head that is a view of
+    another: the result of the contiguous tensors, or a refusal."""
+    g = gen(52)
+    n, heads, kv, d = 150, 8, 4, 128
+    q, k, v = randn(g, n, heads, d, dtype=BF16), randn(g, n, kv, d, dtype=BF16), randn(g, n, kv, d, dtype=BF16)
+    cu = i32([0, 100, n]).cuda()
+    want = attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu)
+
+    def outer(t):  # [heads, tokens, d] in memory
+        return t.transpose(0, 1).contiguous().cuda().transpose(0, 1)
+
+    def gaps(t):
+        wide = torch.full((n, t.shape[1] + 3, d + 24), math.nan, dtype=BF16, device="cuda")
+        wide[:, 1:-2, 8:8 + d] = t.cuda()
+        return wide[:, 1:-2, 8:8 + d]
+
+    out = torch.full((heads, n, d), 7.0, dtype=BF16, device="cuda").transpose(0, 1)
+    for layout in (outer, gaps):
+        assert torch.equal(attention.prefill(layout(q), layout(k), layout(v), cu), want)
+    assert torch.equal(attention.prefill(outer(q), gaps(k), v.cuda(), cu, out=out), want)
+    # one key head for all queries, out of a buffer of several
+    one = attention.prefill(q.cuda(), k.cuda()[:, 2:3], v.cuda()[:, 2:3], cu)
+    R.close(one[:100], *R.attention(q[:100], k[:100, 2:3], v[:100, 2:3]))
+    # a broadcast head
+    try:
+        got = attention.prefill(q.cuda(), k.cuda()[:, 1:2].expand(n, kv, d), v.cuda()[:, 1:2].expand(n, kv, d), cu)
+    except AmoeError as e:
+        assert "strides" in str(e)
+    else:
+        R.close(got[:100], *R.attention(q[:100], k[:100, 1:2].expand(100, kv, d), v[:100, 1:2].expand(100, kv, d)))
+    # rows that do not start on 16 bytes
+    odd = torch.zeros(n, heads, d + 4, dtype=BF16, device="cuda")[:, :, 4:]
+    with pytest.raises(AmoeError, match="16 bytes"):
+        attention.prefill(odd, k.cuda(), v.cuda(), cu)
+    with pytest.raises(AmoeError, match="overlap"):
+        attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu, out=out[:, :1].expand(n, heads, d))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_nan_queries_and_keys(cuda_device, d):
+    """A NaN in one query's row stays there; one in a key's row reaches every later query, whichever column of a tile
+    the key stands in."""
+    g = gen(53)
+    n = 80
+    q, k, v = randn(g, n, 2, d, dtype=F16), randn(g, n, 1, d, dtype=F16), randn(g, n, 1, d, dtype=F16)
+    cu = i32([0, n]).cuda()
+    clean = attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu)
+    bad = q.clone()
+    bad[33, 1, 5] = math.nan
+    got = attention.prefill(bad.cuda(), k.cuda(), v.cuda(), cu)
+    assert torch.isnan(got[33, 1]).all()
+    got[33, 1] = clean[33, 1]
+    assert torch.equal(got, clean)
+    for j in list(range(20)) + [63, 64, 79]:
+        bad = k.clone()
+        bad[j, 0, 3] = math.nan
+        got = attention.prefill(q.cuda(), bad.cuda(), v.cuda(), cu)
+        assert torch.isnan(got[j:]).all(), j
+        assert torch.equal(got[:j], clean[:j]), j
+
+
+def test_prefill_far_sinks_and_windows(cuda_device):
+    g = gen(54)
+    n = 200
+    q, k, v = randn(g, n, 8, 64, dtype=BF16), randn(g, n, 2, 64, dtype=BF16), randn(g, n, 2, 64, dtype=BF16)
+    cu = i32([0, n]).cuda()
+    sinks = torch.tensor([-1e4, 1e4, -300.0, 300.0, 0.0, -math.inf, 60.0, -60.0])
+    out = attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu, sinks=sinks.cuda())
+    R.close(out, *R.attention(q, k, v, sinks))
+    sinks[3] = math.inf
+    out = attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu, sinks=sinks.cuda())
+    assert torch.isnan(out[:, 3]).all() and torch.isfinite(out[:, :3]).all()
+    plain = attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu)
+    for window in (n, n + 1, 2 ** 31 - 1):
+        assert torch.equal(attention.prefill(q.cuda(), k.cuda(), v.cuda(), cu, window=window), plain)
+    # more queries than keys under the longest window
+    out = attention.prefill(q.cuda(), k[:50].cuda(), v[:50].cuda(), cu, i32([0, 50]).cuda(), window=2 ** 31 - 1)
+    assert (out[:150] == 0).all()
+    R.close(out[150:], *R.attention(q[150:], k[:50], v[:50]))
+
+
+def test_a_long_decode_is_captured(cuda_device):
+    """The form with a workspace and a second kernel, in a graph, and its refusal without the workspace."""
+    g = gen(55)
+    cache = attention.KVCache(700, 64, 1, 64, dtype=F16)
+    cache.k.copy_(randn(g, 700, 1, 64, 64)), cache.v.copy_(randn(g, 700, 1, 64, 64))
+    table = torch.randperm(700, generator=g).to(torch.int32).view(1, 700).cuda()
+    q, length = randn(g, 1, 8, 64, dtype=F16).cuda(), i32([40001]).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.decode(q, table, length)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.decode(q, table, length)
+    for n in (40001, 12, 44800):
+        length.fill_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, cache.decode(q, table, length))
+        k, v = (R.rows_of(t.cpu(), None, table[0].cpu(), 0, n) for t in (cache.k, cache.v))
+        R.close(out, *R.attention(q.cpu(), k, v))
+    cache.check()
