@@ -464,11 +464,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free);
-            if (key + N - 1 > at0 || (p.window > 0 && key <= hi - 1 - p.window)) {
-                const int last = at - key, first = p.window > 0 ? at - p.window + 1 - key : 0;
+            if (key + N - 1 > at0) {  // some row's keys end in this tile
+                const int last = at - key;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (i > last || i < first) s[i] = -INFINITY;
+                    if (i > last) s[i] = -INFINITY;
+            }
+            if (p.window > 0 && key <= hi - 1 - p.window) {  // some row's window begins in it
+                const int first = at - p.window + 1 - key;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (i < first) s[i] = -INFINITY;
             }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // chains short enough to overlap
 #pragma unroll
