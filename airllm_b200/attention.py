@@ -313,6 +313,9 @@ class KVCache:
         _invalid("kv cache: " + ", ".join(said))
 
 
+_prefill_workspace: dict = {}
+
+
 def prefill(q, k, v, cu_q, cu_k=None, scale: float | None = None, window: int = 0, sinks=None, out=None,
             stream=None):
     """Causal attention of packed prompts (amoe_attn_prefill): rows cu_q[s]..cu_q[s+1] of q
@@ -332,10 +335,19 @@ def prefill(q, k, v, cu_q, cu_k=None, scale: float | None = None, window: int = 
         out = _like(q, None, st)
     else:
         _written(out, "out")
+    cq, ck = _rows(q, "q", n, d, dev), _rows(k, "k", m, d, dev)
+    shape = (d, window, heads, k.shape[1], n, m, seqs)
+    size = _prefill_workspace.get(shape)
+    if size is None:  # the library's answer for these shapes; what it refuses, the call below refuses too
+        size = max(lib.amoe_attn_prefill_workspace(*shape), 0)
+        if len(_prefill_workspace) > 1000:
+            _prefill_workspace.clear()
+        _prefill_workspace[shape] = size
+    work = _empty(q, size, torch.uint8, st) if size else None
     rc = lib.amoe_attn_prefill(
-        dev, d, _attn(scale, window, sinks, heads, dev), _rows(q, "q", n, d, dev), _rows(k, "k", m, d, dev),
-        _rows(v, "v", m, d, dev), _rows(out, "out", n, d, dev), n, m, _ints(cu_q, "cu_q", seqs + 1, dev),
-        _ints(cu_k, "cu_k", seqs + 1, dev), seqs, raw)
+        dev, d, _attn(scale, window, sinks, heads, dev), cq, ck, _rows(v, "v", m, d, dev),
+        _rows(out, "out", n, d, dev), n, m, _ints(cu_q, "cu_q", seqs + 1, dev), _ints(cu_k, "cu_k", seqs + 1, dev),
+        seqs, None if work is None else work.data_ptr(), size, raw)
     if rc:
         _check(lib, rc)
     return out

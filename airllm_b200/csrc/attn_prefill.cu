@@ -19,7 +19,11 @@
 // 8: 704 us, 780 TFLOP/s, 0.47 of the measured bf16 GEMM.  Two row tiles of one persistent CTA (0.93 ms: fewer warps
 // to hide a tile's chain of waits), two threads a row (0.85 ms: the pair has to agree on its maximum) and P in S's
 // own columns (0.80 ms: Q K^T waits for P V) were slower.  128-wide heads: the tensor cores and the operands they read
-// from shared memory; 1500 tokens behind 8000: 107 us, 680 TFLOP/s.  Windows and short prompts: a CTA's start.
+// from shared memory; 1500 tokens in three chunks behind 2600-2800 each: 107 us, 680 TFLOP/s.  Windows and short
+// prompts: a CTA's start.
+//
+// Few row tiles (a few queries behind many keys) do not fill the GPU: their keys are split over CTAs, and a second kernel
+// joins the partial sums (`layout` below chooses, with what it measured).
 //
 // The maximum is lazy: O and the sum are rescaled only when a row's maximum has grown by more
 // than 2^8 since the last time, which float32 sums and 16-bit weights (relative precision) hold without loss.
@@ -30,6 +34,7 @@
 #include "attn.cuh"
 #include "tc_ptx.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace amoe {
@@ -53,6 +58,8 @@ struct PrefillParams {
     const float *sinks;
     float scale_log2;
     int window, q_tokens, k_tokens, seqs, group, tile_tokens, kv_heads;
+    int split;     // CTAs to a row tile's keys
+    float *work;   // split > 1: partial sums, [tile][part][D + 2][kRows]: each row's O, m and l
 };
 
 template <int D>
@@ -78,7 +85,7 @@ struct Cfg {
 struct Work {
     int tok0, tokens;    // first query row and how many of the tile's are the sequence's
     int at0;             // position of the first among its keys
-    int k0, lo, hi;      // the sequence's first key row; visible keys [lo, hi) of the tile
+    int k0, lo, hi;      // the sequence's first key row; the tile's visible keys [lo, hi), or this CTA's part of them
     int dead;            // a bounded wait gave up
     int found;
 };
@@ -226,8 +233,10 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
 }
 
-// One warp finds the sequence and tile of CTA x: sequences in order, each one's last (longest) tile first.
-__device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w) {
+// One warp finds the sequence and rows of tile x: sequences in order, each one's last (longest) tile first; and of
+// its keys the part-th part (-1: all).
+template <int N>
+__device__ __forceinline__ bool find_work(const PrefillParams &p, int x, int part, Work *w) {
     const int lane = threadIdx.x % 32;
     int before = 0;
     for (int s0 = 0; s0 < p.seqs; s0 += 32) {
@@ -254,6 +263,12 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, Work *w
             w->k0 = k0;
             w->hi = max(w->at0 + w->tokens, 0);
             w->lo = p.window > 0 ? max(w->at0 - p.window + 1, 0) : 0;
+            if (part >= 0 && w->hi > w->lo) {
+                const int tiles = (w->hi - w->lo - 1) / N + 1;
+                const int t0 = (int)((int64_t)tiles * part / p.split), t1 = (int)((int64_t)tiles * (part + 1) / p.split);
+                w->hi = min(w->hi, w->lo + t1 * N);
+                w->lo = min(w->lo + t0 * N, w->hi);
+            }
             w->dead = 0;
         }
         if (__any_sync(0xffffffffu, mine)) return true;
@@ -308,7 +323,9 @@ __device__ __forceinline__ void row_again(const PrefillParams &p, int tok, int h
     }
 }
 
-template <int D, int TYPE>
+// SPLIT: a tile's keys are split over p.split CTAs (windowed calls of many tiles, which a CTA's start bounds, took 4 %
+// longer where one kernel did both).
+template <int D, int TYPE, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
     prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
@@ -324,10 +341,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
     Work *work = reinterpret_cast<Work *>(tmem_slot + 2);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int kvh = blockIdx.x % p.kv_heads;
+    const int part = SPLIT ? (int)(blockIdx.x % p.split) : -1, tile = SPLIT ? blockIdx.x / p.split : blockIdx.x;
+    const int kvh = tile % p.kv_heads;
     // the work is found while the TMEM columns, the barriers and the tensor maps are made ready
     if (warp == 0) {
-        const bool f = find_work(p, blockIdx.x / p.kv_heads, work);
+        const bool f = find_work<N>(p, tile / p.kv_heads, part, work);
         if (lane == 0) work->found = f;
     } else if (warp == 1) {
         if (lane == 0) {
@@ -365,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_p),
                          "n"(C::kTmemP ? C::kTmemP : 32));
     };
+    if (SPLIT) cudaTriggerProgrammaticLaunchCompletion();  // lets the join take the places that fall free
     if (!work->found) {
         leave();
         return;
@@ -470,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                 for (int i = 0; i < N; ++i)
                     if (i > last) s[i] = -INFINITY;
             }
-            if (p.window > 0 && key <= hi - 1 - p.window) {  // some row's window begins in it
+            if (p.window > 0 && key < (SPLIT ? at0 + p.tile_tokens : hi) - p.window) {  // some row's window begins in it
                 const int first = at - p.window + 1 - key;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
@@ -532,39 +551,103 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
-        if (p.sinks && mine) l += sink_weight(p.sinks[head], m == -INFINITY ? 0.0f : m * p.scale_log2);
-        // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
-        const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
-        char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
-        float worst = isnan(l) ? l : 0.0f;  // 0, or NaN
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-            float o[32];
-            __syncwarp();
-            if (tiles > 0) {
-                bs::tmem_ld32(tmem + lanes + C::kO + c, o);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        if constexpr (SPLIT) {  // the row's sums over this part, for the kernel that joins them
+            float *sums = p.work + (int64_t)(tile * p.split + part) * (D + 2) * kRows + r;
+            if (mine) {
+                sums[D * kRows] = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+                sums[(D + 1) * kRows] = ok ? l : NAN;
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;
-            if (mine) {
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                __syncwarp();
+                if (tiles > 0) bs::tmem_ld32(tmem + lanes + C::kO + c, o);
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    float x[8];
+                for (int i = 0; i < 32; ++i)
+                    if (mine) sums[(c + i) * kRows] = tiles > 0 ? o[i] : 0.0f;
+            }
+        } else {
+            if (p.sinks && mine) l += sink_weight(p.sinks[head], m == -INFINITY ? 0.0f : m * p.scale_log2);
+            // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
+            const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
+            char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
+            float worst = isnan(l) ? l : 0.0f;  // 0, or NaN
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = o[i + e] * by;
-                    store8<TYPE>(dst + (c + i) * 2, x);
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                __syncwarp();
+                if (tiles > 0) {
+                    bs::tmem_ld32(tmem + lanes + C::kO + c, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = o[i + e] * by;
+                        store8<TYPE>(dst + (c + i) * 2, x);
+                    }
                 }
             }
+            if (mine && ok && worst != 0.0f)
+                row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
         }
-        if (mine && ok && worst != 0.0f)
-            row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
     }
     tc_fence_before();
     __syncthreads();
     leave();
+}
+
+// The join of the parts' sums.  A CTA takes 32 rows of a tile, a lane a row, a warp eight of the row's elements: sums are
+// read along the rows, as they were written, and a thread's loads do not wait for one another.
+constexpr int kJoinBlocks = kRows / 32;
+template <int D, int TYPE>
+__global__ void __launch_bounds__(D * 4) prefill_join_kernel(const __grid_constant__ PrefillParams p) {
+    __shared__ Work work;
+    __shared__ int again[32];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tile = blockIdx.x / kJoinBlocks, kvh = tile % p.kv_heads;
+    if (warp == 0) {
+        const bool f = find_work<Cfg<D>::N>(p, tile / p.kv_heads, -1, &work);
+        if (lane == 0) work.found = f;
+        again[lane] = 0;
+    }
+    __syncthreads();
+    if (!work.found) return;
+    cudaGridDependencySynchronize();  // launched while the partial sums are still being made
+    const int r = blockIdx.x % kJoinBlocks * 32 + lane, tok = r / p.group, head = kvh * p.group + r % p.group;
+    if (r < work.tokens * p.group) {
+        const int64_t step = (D + 2) * kRows;
+        const float *sums = p.work + tile * p.split * step + r;
+        float top = -INFINITY;
+#pragma unroll 8
+        for (int i = 0; i < p.split; ++i) top = fmaxf(top, sums[i * step + D * kRows]);
+        const float z = top == -INFINITY ? 0.0f : top;
+        float l = 0.0f, o[8] = {};
+#pragma unroll 4
+        for (int i = 0; i < p.split; ++i) {
+            const float *part = sums + i * step, by = ex2(part[D * kRows] - z);
+            l += by * part[(D + 1) * kRows];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] += by * part[(warp * 8 + e) * kRows];
+        }
+        if (p.sinks) l += sink_weight(p.sinks[head], z);
+        const float by = top == -INFINITY ? 0.0f : 1.0f / l;
+        float worst = isnan(l) ? l : 0.0f;  // 0, or NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) worst += o[e] * 0.0f, o[e] *= by;
+        store8<TYPE>(p.out.p + (int64_t)(work.tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + warp * 16, o);
+        if (worst != 0.0f) again[lane] = 1;
+    }
+    __syncthreads();
+    if (warp == 0 && again[lane]) {
+        const int at = work.at0 + tok;
+        row_again<D, TYPE>(p, work.tok0 + tok, head, work.k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
+    }
 }
 
 // [tokens][heads][D] rows as a 3-D map with boxes of 64 elements x heads x tokens.
@@ -582,20 +665,68 @@ bool encode_rows(CUtensorMap *tm, const amoe_rows *r, int D, int tokens, int box
 }
 
 constexpr int kMaxDevices = 64;
+constexpr int kSms = 148;
 constexpr int kMaxTokens = 1 << 30;  // row indexes and positions stay far inside 32 bits
 
 template <int D, int TYPE>
 cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const PrefillParams &p, int device,
                    dim3 grid, cudaStream_t st) {
-    auto *kernel = prefill_kernel<D, TYPE>;
-    static std::atomic<bool> ready[kMaxDevices];
+    auto *kernel = p.split > 1 ? prefill_kernel<D, TYPE, true> : prefill_kernel<D, TYPE, false>;
+    static std::atomic<bool> done[2][kMaxDevices];
+    std::atomic<bool> *ready = done[p.split > 1];
     if (!ready[device].load(std::memory_order_acquire)) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
         if (e != cudaSuccess) return e;
         ready[device].store(true, std::memory_order_release);
     }
     kernel<<<grid, kThreads, Cfg<D>::kSmem, st>>>(q, k, v, p);
-    return cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || p.split == 1) return e;
+    cudaLaunchConfig_t join{};
+    join.gridDim = dim3(grid.x / p.split * kJoinBlocks);
+    join.blockDim = dim3(D * 4);
+    join.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    join.attrs = attr;
+    join.numAttrs = 1;
+    return cudaLaunchKernelEx(&join, prefill_join_kernel<D, TYPE>, p);
+}
+
+// How a call is laid out: row tiles of all kv heads, CTAs to a tile's keys, and the workspace of more than one.
+struct Layout {
+    int64_t tiles;
+    int split;
+    int64_t bytes;
+};
+
+// Few row tiles leave SMs idle, or the last of their waves does, and a tile's keys are then split.  The split is the one of
+// the least expected time: a CTA takes 1 us for 64 keys however many share its SM, and 4 us to start and end; the
+// join takes 3 us, 1/4 us a part that its threads walk, and the partial sums' way through L2 15 ns (64-wide heads) or
+// 30 ns a CTA.  Measured, one CTA a tile -> split (64/8 heads of 64): 16 queries behind 2048 keys 29 -> 12.6 us in 8
+// parts (14.4 in 16), behind 32768 460 -> 37 us in 32; 512 behind 8192 129 -> 120 us in 3; 128 behind none 6.0 us, in 2
+// parts 8.9.  32/8 heads of 128: 64 behind 8192 134 -> 31 us; 300 behind 3000 55 -> 32 us in 3 (39 in 4).
+constexpr int kMaxSplit = 32;
+Layout layout(int head_dim, int window, int64_t q_tokens, int64_t k_tokens, int64_t seqs, int q_heads, int kv_heads) {
+    const int tile_tokens = kRows / (q_heads / kv_heads);
+    // every sequence's last tile may hold a single token
+    const int64_t tiles = (q_tokens + std::min(seqs, q_tokens) * (tile_tokens - 1)) / tile_tokens * kv_heads;
+    Layout l{tiles, 1, 0};
+    int64_t keys = k_tokens / seqs;  // the host knows no sequence's own length
+    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + tile_tokens);
+    const int64_t slots = kSms * (head_dim == 64 ? Cfg<64>::kCtas : Cfg<128>::kCtas);
+    const int64_t steps = (keys + 63) / 64;
+    float best = 0.0f;
+    // no more than four waves: the partial sums (34 or 67 KB a CTA) stay in L2
+    for (int64_t s = 1; s <= kMaxSplit && s <= steps && (s == 1 || tiles * s <= 4 * slots); ++s) {
+        float us = (float)((tiles * s + slots - 1) / slots * ((steps + s - 1) / s + 4));
+        if (s > 1) us += 3.0f + 0.25f * s + (head_dim == 64 ? 0.015f : 0.03f) * (tiles * s);
+        if (s == 1) best = us * 0.95f;  // a split has to gain something
+        else if (us < best) best = us, l.split = (int)s;
+    }
+    if (l.split > 1) l.bytes = tiles * l.split * kRows * (head_dim + 2) * 4;
+    return l;
 }
 
 }  // namespace
@@ -605,10 +736,21 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
 using namespace amoe;
 using namespace amoe::attn;
 
-extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, const amoe_rows *q,
-                                 const amoe_rows *k, const amoe_rows *v, const amoe_rows *out, int32_t q_tokens,
-                                 int32_t k_tokens, const int32_t *cu_q, const int32_t *cu_k, int32_t seqs,
-                                 void *stream) {
+extern "C" {
+
+int64_t amoe_attn_prefill_workspace(int32_t head_dim, int32_t window, int32_t q_heads, int32_t kv_heads,
+                                    int32_t q_tokens, int32_t k_tokens, int32_t seqs) {
+    if (int rc = check_head_dim(head_dim)) return rc;
+    if (int rc = check_group(q_heads, kv_heads)) return rc;
+    if (window < 0 || q_tokens < 0 || k_tokens < 0 || seqs < 1)
+        return reject("window, q_tokens and k_tokens must not be negative, seqs must be positive");
+    return layout(head_dim, window, q_tokens, k_tokens, seqs, q_heads, kv_heads).bytes;
+}
+
+int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, const amoe_rows *q, const amoe_rows *k,
+                      const amoe_rows *v, const amoe_rows *out, int32_t q_tokens, int32_t k_tokens,
+                      const int32_t *cu_q, const int32_t *cu_k, int32_t seqs, void *workspace,
+                      int64_t workspace_bytes, void *stream) {
     if (int rc = check_attn(attn)) return rc;
     if (int rc = check_head_dim(head_dim)) return rc;
     if (q_tokens < 0 || k_tokens < 0) return reject("q_tokens and k_tokens must not be negative");
@@ -633,9 +775,13 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
     p.group = q->heads / k->heads;
     p.tile_tokens = kRows / p.group;
     p.kv_heads = k->heads;
-    // every sequence's last tile may be a short one
-    const int64_t ctas = ((int64_t)q_tokens / p.tile_tokens + (seqs < q_tokens ? seqs : q_tokens)) * k->heads;
-    if (ctas > INT_MAX) return reject("too many query rows");
+    const Layout l = layout(head_dim, attn->window, q_tokens, k_tokens, seqs, q->heads, k->heads);
+    if (l.tiles * l.split > INT_MAX) return reject("too many query rows");
+    if (l.split > 1 && (!workspace || workspace_bytes < l.bytes))
+        return reject("prefill needs a workspace of " + std::to_string(l.bytes) + " bytes");
+    if (l.split > 1 && (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return reject("workspace must be 16-byte aligned");
+    p.split = l.split, p.work = static_cast<float *>(workspace);
     DeviceScope scope;
     cudaError_t e = scope.enter(device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
@@ -649,7 +795,8 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
         !encode_rows(&tk, k, head_dim, k_tokens, 1, n) || !encode_rows(&tv, v, head_dim, k_tokens, 1, n))
         return reject("prefill: strides of q, k or v that a tensor map cannot take");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)ctas);  // kv heads first, then a sequence's tiles from the longest down
+    // parts first, then kv heads, then a sequence's tiles from the longest down
+    const dim3 grid((unsigned)(l.tiles * l.split));
     if (head_dim == 64)
         e = q->type == AMOE_GGUF_F16 ? launch<64, AMOE_GGUF_F16>(tq, tk, tv, p, device, grid, st)
                                      : launch<64, AMOE_GGUF_BF16>(tq, tk, tv, p, device, grid, st);
@@ -658,3 +805,5 @@ extern "C" int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_at
                                      : launch<128, AMOE_GGUF_BF16>(tq, tk, tv, p, device, grid, st);
     return e == cudaSuccess ? AMOE_OK : cuda_error(e, "prefill kernel");
 }
+
+}  // extern "C"

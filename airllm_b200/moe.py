@@ -124,7 +124,9 @@ SIGNATURES = {
     "amoe_rope_init": (ctypes.c_int, [_i32, ctypes.c_double, _i32, _vp]),
     "amoe_kv_append": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "amoe_kv_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
-    "amoe_attn_prefill": (ctypes.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "amoe_attn_prefill": (ctypes.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp,
+                                         ctypes.c_int64, _vp]),
+    "amoe_attn_prefill_workspace": (ctypes.c_int64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "amoe_attn_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, ctypes.c_int64, _vp]),
     "amoe_attn_decode_workspace": (ctypes.c_int64, [_vp, _vp, _i32, _i32, _i32]),
 }

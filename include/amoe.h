@@ -412,12 +412,20 @@ typedef struct amoe_attn {
  * the softmax's maximum and sum are float32, its weights rounded to that type.  q_tokens and
  * k_tokens (at most 2^30) are the rows given; rows of out from cu_q[seqs] on are left as they
  * are, and starts that decrease or pass the rows given are clamped to them.  Strides must be
- * such as a CUDA tensor map takes.  A wait inside the kernel that gives up after about a
- * second leaves NaN rows. */
+ * such as a CUDA tensor map takes.  workspace: amoe_attn_prefill_workspace's bytes of device
+ * memory (NULL where that is 0), 16-byte aligned, the call's own until it has run; its
+ * contents before and after mean nothing.  A wait inside the kernel that gives up after about a
+ * second leaves NaN rows, or rows that took long. */
 AMOE_API int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, const amoe_rows *q,
                                const amoe_rows *k, const amoe_rows *v, const amoe_rows *out, int32_t q_tokens,
                                int32_t k_tokens, const int32_t *cu_q, const int32_t *cu_k, int32_t seqs,
-                               void *stream);
+                               void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that amoe_attn_prefill needs for these shapes (no GPU needed), 0 where one
+ * launch does; negative: an error.  A few queries behind many keys need one: up to 32 CTAs
+ * then share the keys of 128 rows. */
+AMOE_API int64_t amoe_attn_prefill_workspace(int32_t head_dim, int32_t window, int32_t q_heads, int32_t kv_heads,
+                                             int32_t q_tokens, int32_t k_tokens, int32_t seqs);
 
 /* The same for one new token a sequence, over the cache: row s of q and out is the query at
  * position kv_len[s] - 1 of sequence s (kv_len [seqs], device, the new token included; 0: a

@@ -111,12 +111,12 @@ def test_prefill_refusals(kw, word):
     a = moe.AmoeAttn(kw.get("scale", 0.0), kw.get("window", 0), None)
     q, k, v, o = (kw.get(n, rows()) for n in "qkvo")
     refused(lib.amoe_attn_prefill(0, kw.get("d", 64), ref(a), ref(q), ref(k), ref(v), ref(o), kw.get("n", 5), 5,
-                                  kw.get("cu", AT), AT, kw.get("seqs", 1), None), word)
+                                  kw.get("cu", AT), AT, kw.get("seqs", 1), None, 0, None), word)
 
 
 def test_prefill_without_rows_does_nothing():
     lib, r, a = moe.load_library(), rows(), moe.AmoeAttn(0.0, 0, None)
-    assert lib.amoe_attn_prefill(0, 64, ref(a), ref(r), ref(r), ref(r), ref(r), 0, 5, AT, AT, 1, None) == moe.AMOE_OK
+    assert lib.amoe_attn_prefill(0, 64, ref(a), ref(r), ref(r), ref(r), ref(r), 0, 5, AT, AT, 1, None, 0, None) == moe.AMOE_OK
 
 
 @pytest.mark.parametrize("c,q,o,kw,word", [
@@ -177,3 +177,20 @@ def test_index_arithmetic_stays_in_bounds(tmp_path):
                     os.path.join(CUDA, "kv_index_check.cu")], check=True)
     got = subprocess.run([exe], capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout.strip() == "ok", got.stdout
+
+
+def test_prefill_workspace():
+    lib, a, r = moe.load_library(), moe.AmoeAttn(0.0, 0, None), rows()
+    def size(d=64, window=0, heads=8, kv=8, q=16, k=32768, n=1):
+        return lib.amoe_attn_prefill_workspace(d, window, heads, kv, q, k, n)
+    # few queries behind many keys need one; many queries, few keys, a window or many sequences none
+    assert size() > 0 and size(d=128) > 0 and size(q=1) > 0
+    assert size(q=20000) == 0 and size(k=200) == 0 and size(window=128) == 0 and size(q=300, n=300) == 0
+    assert size(q=0, k=0) == 0
+    for bad in (dict(d=80), dict(heads=12), dict(window=-1), dict(q=-1), dict(k=-1), dict(n=0)):
+        assert size(**bad) == moe.AMOE_ERR_INVALID
+    for work, n in ((None, size()), (AT, size() - 1)):
+        refused(lib.amoe_attn_prefill(0, 64, ref(a), ref(r), ref(r), ref(r), ref(r), 16, 32768, AT, AT, 1, work, n, None),
+                "workspace")
+    refused(lib.amoe_attn_prefill(0, 64, ref(a), ref(r), ref(r), ref(r), ref(r), 16, 32768, AT, AT, 1, AT + 4, 1 << 40,
+                                  None), "aligned")

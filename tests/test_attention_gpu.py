@@ -8,7 +8,7 @@ import torch
 
 import attention_ref as R
 import oracle
-from airllm_b200 import AmoeError, attention
+from airllm_b200 import AmoeError, attention, moe
 
 pytestmark = pytest.mark.gpu
 E4M3 = torch.float8_e4m3fn
@@ -734,3 +734,70 @@ def test_a_long_decode_is_captured(cuda_device):
         k, v = (R.rows_of(t.cpu(), None, table[0].cpu(), 0, n) for t in (cache.k, cache.v))
         R.close(out, *R.attention(q.cpu(), k, v))
     cache.check()
+
+
+SPLITS = [  # queries, keys before them, heads, kv_heads, d, type, window, sinks: few rows behind many keys
+    ([1], [5000], 64, 8, 64, BF16, 0, True),
+    ([17], [8191], 8, 1, 64, F16, 0, False),
+    ([40], [3001], 8, 2, 128, BF16, 0, True),
+    ([3, 0, 20], [9000, 100, 10], 12, 1, 64, BF16, 0, True),
+    ([33], [7000], 10, 2, 128, F16, 2100, False),
+    ([9], [20000], 128, 1, 64, F16, 0, True),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SPLITS)))
+def test_prefill_split_over_the_keys(cuda_device, case):
+    new, before, heads, kv, d, dtype, window, with_sinks = SPLITS[case]
+    g = gen(300 + case)
+    keys = [a + b for a, b in zip(new, before)]
+    n, m = sum(new), sum(keys)
+    assert moe.load_library().amoe_attn_prefill_workspace(d, window, heads, kv, n + 2, m, len(new)) > 0
+    q = randn(g, n + 2, heads, d, dtype=dtype, scale=2.0)
+    k, v = randn(g, m, kv, d, dtype=dtype), randn(g, m, kv, d, dtype=dtype)
+    sinks = randn(g, heads, scale=2.0) if with_sinks else None
+    # beside the plain values: an infinity that only the last query of the first sequence sees, NaN behind the first
+    # sequence's keys where there is another
+    bad = v.clone()
+    if new[0] > 1:
+        bad[keys[0] - 1, 0, 3] = math.inf
+    if len(new) > 1:
+        bad[keys[0]:keys[0] + keys[1]] = math.nan
+    for values in (v, bad):
+        out = torch.full((n + 2, heads, d), 7.0, dtype=dtype, device="cuda")
+        attention.prefill(q.cuda(), k.cuda(), values.cuda(), starts(new).cuda(), starts(keys).cuda(), window=window,
+                          sinks=None if sinks is None else sinks.cuda(), out=out)
+        assert (out[n:] == 7).all()
+        a = b = 0
+        for x, y in zip(new, keys):
+            want, bound = R.attention(q[a:a + x], k[b:b + y], values[b:b + y], sinks, window)
+            got = out[a:a + x].double().cpu()
+            fine = torch.isfinite(want)
+            assert torch.equal(torch.isfinite(got), fine)
+            assert ((got - want).abs()[fine] <= bound[fine]).all()
+            a, b = a + x, b + y
+
+
+def test_a_split_prefill_is_captured_and_sees_nothing(cuda_device):
+    g = gen(310)
+    q = randn(g, 30, 8, 64, dtype=BF16).cuda()
+    k, v = randn(g, 6000, 1, 64, dtype=BF16).cuda(), randn(g, 6000, 1, 64, dtype=BF16).cuda()
+    cu_q, cu_k = i32([0, 30]).cuda(), i32([0, 6000]).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attention.prefill(q, k, v, cu_q, cu_k)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attention.prefill(q, k, v, cu_q, cu_k)
+    for n in (6000, 0, 7, 3333):
+        cu_k[1] = n
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        # queries that stand before every key see nothing
+        seen = min(n, 30)
+        assert (out[:30 - seen] == 0).all()
+        if seen:
+            R.close(out[30 - seen:], *R.attention(q[30 - seen:].cpu(), k[:n].cpu(), v[:n].cpu()))
