@@ -19,11 +19,11 @@
 // 8: 704 us, 780 TFLOP/s, 0.47 of the measured bf16 GEMM.  Two row tiles of one persistent CTA (0.93 ms: fewer warps
 // to hide a tile's chain of waits), two threads a row (0.85 ms: the pair has to agree on its maximum) and P in S's
 // own columns (0.80 ms: Q K^T waits for P V) were slower.  128-wide heads: the tensor cores and the operands they read
-// from shared memory; 1500 tokens in three chunks behind 2600-2800 each: 107 us, 680 TFLOP/s.  Windows and short
+// from shared memory; 1500 tokens in three chunks behind 2600-2800 each: 87 us, 835 TFLOP/s.  Windows and short
 // prompts: a CTA's start.
 //
-// Few row tiles (a few queries behind many keys) do not fill the GPU: their keys are split over CTAs, and a second kernel
-// joins the partial sums (`layout` below chooses, with what it measured).
+// A few queries behind many keys, or the last wave of a larger call, do not fill the GPU: the keys of those tiles are
+// split over CTAs, and a second kernel joins the partial sums (`layout` below chooses, with what it measured).
 //
 // The maximum is lazy: O and the sum are rescaled only when a row's maximum has grown by more
 // than 2^8 since the last time, which float32 sums and 16-bit weights (relative precision) hold without loss.
@@ -58,8 +58,9 @@ struct PrefillParams {
     const float *sinks;
     float scale_log2;
     int window, q_tokens, k_tokens, seqs, group, tile_tokens, kv_heads;
-    int split;     // CTAs to a row tile's keys
-    float *work;   // split > 1: partial sums, [tile][part][D + 2][kRows]: each row's O, m and l
+    int whole;    // row tiles (of all kv heads) that one CTA takes; those behind them have
+    int split;    // so many CTAs to their keys
+    float *work;  // split > 1: their partial sums, [tile][part][D + 2][kRows]: each row's O, m and l
 };
 
 template <int D>
@@ -323,7 +324,7 @@ __device__ __forceinline__ void row_again(const PrefillParams &p, int tok, int h
     }
 }
 
-// SPLIT: a tile's keys are split over p.split CTAs (windowed calls of many tiles, which a CTA's start bounds, took 4 %
+// SPLIT: the keys of tiles from p.whole on are split over p.split CTAs (windowed calls of many tiles, which a CTA's start bounds, took 4 %
 // longer where one kernel did both).
 template <int D, int TYPE, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
@@ -341,7 +342,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
     Work *work = reinterpret_cast<Work *>(tmem_slot + 2);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int part = SPLIT ? (int)(blockIdx.x % p.split) : -1, tile = SPLIT ? blockIdx.x / p.split : blockIdx.x;
+    int tile = blockIdx.x, part = -1;
+    if (SPLIT && tile >= p.whole) {
+        part = (tile - p.whole) % p.split;
+        tile = p.whole + (tile - p.whole) / p.split;
+    }
     const int kvh = tile % p.kv_heads;
     // the work is found while the TMEM columns, the barriers and the tensor maps are made ready
     if (warp == 0) {
@@ -551,8 +556,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
-        if constexpr (SPLIT) {  // the row's sums over this part, for the kernel that joins them
-            float *sums = p.work + (int64_t)(tile * p.split + part) * (D + 2) * kRows + r;
+        if (SPLIT && part >= 0) {  // the row's sums over this part, for the kernel that joins them
+            float *sums = p.work + (int64_t)((tile - p.whole) * p.split + part) * (D + 2) * kRows + r;
             if (mine) {
                 sums[D * kRows] = m == -INFINITY ? -INFINITY : m * p.scale_log2;
                 sums[(D + 1) * kRows] = ok ? l : NAN;
@@ -610,7 +615,8 @@ template <int D, int TYPE>
 __global__ void __launch_bounds__(D * 4) prefill_join_kernel(const __grid_constant__ PrefillParams p) {
     __shared__ Work work;
     __shared__ int again[32];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tile = blockIdx.x / kJoinBlocks, kvh = tile % p.kv_heads;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int tile = p.whole + blockIdx.x / kJoinBlocks, kvh = tile % p.kv_heads;
     if (warp == 0) {
         const bool f = find_work<Cfg<D>::N>(p, tile / p.kv_heads, -1, &work);
         if (lane == 0) work.found = f;
@@ -622,7 +628,7 @@ __global__ void __launch_bounds__(D * 4) prefill_join_kernel(const __grid_consta
     const int r = blockIdx.x % kJoinBlocks * 32 + lane, tok = r / p.group, head = kvh * p.group + r % p.group;
     if (r < work.tokens * p.group) {
         const int64_t step = (D + 2) * kRows;
-        const float *sums = p.work + tile * p.split * step + r;
+        const float *sums = p.work + (tile - p.whole) * p.split * step + r;
         float top = -INFINITY;
 #pragma unroll 8
         for (int i = 0; i < p.split; ++i) top = fmaxf(top, sums[i * step + D * kRows]);
@@ -683,7 +689,7 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || p.split == 1) return e;
     cudaLaunchConfig_t join{};
-    join.gridDim = dim3(grid.x / p.split * kJoinBlocks);
+    join.gridDim = dim3((grid.x - p.whole) / p.split * kJoinBlocks);
     join.blockDim = dim3(D * 4);
     join.stream = st;
     cudaLaunchAttribute attr[1];
@@ -694,38 +700,45 @@ cudaError_t launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap
     return cudaLaunchKernelEx(&join, prefill_join_kernel<D, TYPE>, p);
 }
 
-// How a call is laid out: row tiles of all kv heads, CTAs to a tile's keys, and the workspace of more than one.
+// How a call is laid out: row tiles of all kv heads, how many of them one CTA takes, CTAs to the keys of each of the
+// others, and the workspace of more than one.
 struct Layout {
-    int64_t tiles;
+    int64_t tiles, whole;
     int split;
     int64_t bytes;
 };
 
-// Few row tiles leave SMs idle, or the last of their waves does, and a tile's keys are then split.  The split is the one of
-// the least expected time: a CTA takes 1 us for 64 keys however many share its SM, and 4 us to start and end; the
-// join takes 3 us, 1/4 us a part that its threads walk, and the partial sums' way through L2 15 ns (64-wide heads) or
-// 30 ns a CTA.  Measured, one CTA a tile -> split (64/8 heads of 64): 16 queries behind 2048 keys 29 -> 12.6 us in 8
-// parts (14.4 in 16), behind 32768 460 -> 37 us in 32; 512 behind 8192 129 -> 120 us in 3; 128 behind none 6.0 us, in 2
-// parts 8.9.  32/8 heads of 128: 64 behind 8192 134 -> 31 us; 300 behind 3000 55 -> 32 us in 3 (39 in 4).
+// The tiles behind the last whole wave of CTAs (all, where they fill none) leave SMs idle, and their keys are then
+// split.  The split is the one of the least expected time: a CTA takes 1 us for 64 keys however many share its SM, and
+// 4 us to start and end; the join takes 3 us, 1/4 us a part that its threads walk, and the partial sums' way through
+// L2 15 ns (64-wide heads) or 30 ns a CTA.  Measured, one CTA a tile -> split (64/8 heads of 64): 16 queries behind
+// 2048 keys 29 -> 12.6 us in 8 parts (14.4 in 16), behind 32768 460 -> 37 us in 32; 512 behind 8192 129 -> 120 us in 3;
+// 128 behind none 6.0 us, in 2 parts 8.9.  32/8 heads of 128: 64 behind 8192 134 -> 31 us; 300 behind 3000 55 -> 32 us
+// in 3 (39 in 4); 1500 behind 8000 (296 whole tiles, 80 split) 256 -> 206 us in 3 (216 in 4; all tiles in 3: 233); 1400
+// behind none 27.5 us, its last tiles in 2 parts 33.
 constexpr int kMaxSplit = 32;
 Layout layout(int head_dim, int window, int64_t q_tokens, int64_t k_tokens, int64_t seqs, int q_heads, int kv_heads) {
     const int tile_tokens = kRows / (q_heads / kv_heads);
     // every sequence's last tile may hold a single token
     const int64_t tiles = (q_tokens + std::min(seqs, q_tokens) * (tile_tokens - 1)) / tile_tokens * kv_heads;
-    Layout l{tiles, 1, 0};
-    int64_t keys = k_tokens / seqs;  // the host knows no sequence's own length
-    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + tile_tokens);
     const int64_t slots = kSms * (head_dim == 64 ? Cfg<64>::kCtas : Cfg<128>::kCtas);
-    const int64_t steps = (keys + 63) / 64;
-    float best = 0.0f;
-    // no more than four waves: the partial sums (34 or 67 KB a CTA) stay in L2
-    for (int64_t s = 1; s <= kMaxSplit && s <= steps && (s == 1 || tiles * s <= 4 * slots); ++s) {
-        float us = (float)((tiles * s + slots - 1) / slots * ((steps + s - 1) / s + 4));
-        if (s > 1) us += 3.0f + 0.25f * s + (head_dim == 64 ? 0.015f : 0.03f) * (tiles * s);
-        if (s == 1) best = us * 0.95f;  // a split has to gain something
-        else if (us < best) best = us, l.split = (int)s;
+    const int64_t whole = tiles / slots * slots, rest = tiles - whole;
+    Layout l{tiles, tiles, 1, 0};
+    // The host knows no sequence's own length and takes them as equal.  A sequence's first tokens come last and
+    // see the fewest keys.
+    const int64_t most = window > 0 ? (int64_t)window + tile_tokens : INT_MAX, keys = k_tokens / seqs;
+    const int64_t before = std::max<int64_t>(keys - q_tokens / seqs, 0);
+    const int64_t steps = (std::min(keys, most) + 63) / 64;
+    const int64_t last = (std::min({keys, most, before + (rest + kv_heads - 1) / kv_heads * tile_tokens}) + 63) / 64;
+    const float full = (float)(whole / slots * (steps + 4));
+    float best = 0.95f * (full + last + 4);  // a split has to gain something
+    // no more than four waves of parts: the partial sums (34 or 67 KB a CTA) stay in L2
+    for (int64_t s = 2; s <= kMaxSplit && s <= last && rest * s <= 4 * slots; ++s) {
+        const float us = full + (rest * s + slots - 1) / slots * ((last + s - 1) / s + 4) + 3.0f + 0.25f * s +
+                         (head_dim == 64 ? 0.015f : 0.03f) * (rest * s);
+        if (us < best) best = us, l.whole = whole, l.split = (int)s;
     }
-    if (l.split > 1) l.bytes = tiles * l.split * kRows * (head_dim + 2) * 4;
+    if (l.split > 1) l.bytes = rest * l.split * kRows * (head_dim + 2) * 4;
     return l;
 }
 
@@ -776,12 +789,12 @@ int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, c
     p.tile_tokens = kRows / p.group;
     p.kv_heads = k->heads;
     const Layout l = layout(head_dim, attn->window, q_tokens, k_tokens, seqs, q->heads, k->heads);
-    if (l.tiles * l.split > INT_MAX) return reject("too many query rows");
+    if (l.tiles > INT_MAX / 2) return reject("too many query rows");
     if (l.split > 1 && (!workspace || workspace_bytes < l.bytes))
         return reject("prefill needs a workspace of " + std::to_string(l.bytes) + " bytes");
     if (l.split > 1 && (reinterpret_cast<uintptr_t>(workspace) & 15))
         return reject("workspace must be 16-byte aligned");
-    p.split = l.split, p.work = static_cast<float *>(workspace);
+    p.whole = (int)l.whole, p.split = l.split, p.work = static_cast<float *>(workspace);
     DeviceScope scope;
     cudaError_t e = scope.enter(device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
@@ -795,8 +808,8 @@ int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, c
         !encode_rows(&tk, k, head_dim, k_tokens, 1, n) || !encode_rows(&tv, v, head_dim, k_tokens, 1, n))
         return reject("prefill: strides of q, k or v that a tensor map cannot take");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // parts first, then kv heads, then a sequence's tiles from the longest down
-    const dim3 grid((unsigned)(l.tiles * l.split));
+    // kv heads first, then a sequence's tiles from the longest down; a split tile's parts before those
+    const dim3 grid((unsigned)(l.whole + (l.tiles - l.whole) * l.split));
     if (head_dim == 64)
         e = q->type == AMOE_GGUF_F16 ? launch<64, AMOE_GGUF_F16>(tq, tk, tv, p, device, grid, st)
                                      : launch<64, AMOE_GGUF_BF16>(tq, tk, tv, p, device, grid, st);

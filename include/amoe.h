@@ -422,8 +422,8 @@ AMOE_API int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn
                                void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Bytes of workspace that amoe_attn_prefill needs for these shapes (no GPU needed), 0 where one
- * launch does; negative: an error.  A few queries behind many keys need one: up to 32 CTAs
- * then share the keys of 128 rows. */
+ * launch does; negative: an error.  A few queries behind many keys need one, and calls whose last
+ * CTAs would leave the GPU idle: up to 32 CTAs then share the keys of 128 rows. */
 AMOE_API int64_t amoe_attn_prefill_workspace(int32_t head_dim, int32_t window, int32_t q_heads, int32_t kv_heads,
                                              int32_t q_tokens, int32_t k_tokens, int32_t seqs);
 

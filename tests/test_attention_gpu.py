@@ -743,6 +743,10 @@ SPLITS = [  # queries, keys before them, heads, kv_heads, d, type, window, sinks
     ([3, 0, 20], [9000, 100, 10], 12, 1, 64, BF16, 0, True),
     ([33], [7000], 10, 2, 128, F16, 2100, False),
     ([9], [20000], 128, 1, 64, F16, 0, True),
+    # more tiles than CTAs that run at once (296, 444): those of the last wave are split
+    ([300], [1500], 128, 1, 128, F16, 0, True),
+    ([250, 210], [700, 1400], 128, 1, 64, BF16, 0, True),
+    ([130, 0, 190], [1900, 100, 1500], 128, 1, 128, BF16, 1200, False),
 ]
 
 
