@@ -623,8 +623,10 @@ __global__ void __launch_bounds__(D * 4) prefill_join_kernel(const __grid_consta
         again[lane] = 0;
     }
     __syncthreads();
+    // Launched while the partial sums are still being made.  CTAs without work wait as well: what follows on the stream waits
+    // for this grid only, which must not end before the other.
+    cudaGridDependencySynchronize();
     if (!work.found) return;
-    cudaGridDependencySynchronize();  // launched while the partial sums are still being made
     const int r = blockIdx.x % kJoinBlocks * 32 + lane, tok = r / p.group, head = kvh * p.group + r % p.group;
     if (r < work.tokens * p.group) {
         const int64_t step = (D + 2) * kRows;

@@ -782,6 +782,23 @@ def test_prefill_split_over_the_keys(cuda_device, case):
             a, b = a + x, b + y
 
 
+def test_a_split_prefill_without_a_split_tile_is_waited_for(cuda_device):
+    # the rows given allow a last wave of split tiles; the starts leave only whole ones, and what follows reads their rows
+    g = gen(309)
+    n, m = 280, 6000
+    q = randn(g, 310, 128, 128, dtype=F16, scale=2.0).cuda()
+    k, v = randn(g, m, 1, 128, dtype=F16).cuda(), randn(g, m, 1, 128, dtype=F16).cuda()
+    assert moe.load_library().amoe_attn_prefill_workspace(128, 0, 128, 1, 310, m, 1) > 0
+    want = attention.prefill(q[:n], k, v, i32([0, n]).cuda(), i32([0, m]).cuda())
+    assert moe.load_library().amoe_attn_prefill_workspace(128, 0, 128, 1, n, m, 1) == 0
+    cu_q, cu_k = i32([0, n]).cuda(), i32([0, m]).cuda()
+    for _ in range(5):
+        out = torch.full_like(q, 7.0)
+        attention.prefill(q, k, v, cu_q, cu_k, out=out)
+        copy = out.clone()
+        assert torch.equal(copy[:n], want) and (copy[n:] == 7).all()
+
+
 def test_a_split_prefill_is_captured_and_sees_nothing(cuda_device):
     g = gen(310)
     q = randn(g, 30, 8, 64, dtype=BF16).cuda()
