@@ -8,9 +8,11 @@
 // c and s = cos, sin (angle) * concentration.  Angles of far positions lose float32, and a
 // value that lands next to a rounding border of the cache's type must fall on the side the
 // definition says, so angles, sines and products are float64 as in the reference, rounded
-// once to float32 (its stored type) and from there to the cache's.  One to four warps take a token:
+// once to float32 (its stored type) and from there to the cache's.  A warp or four take a token:
 // their lanes compute the angles, then d/16 lanes a head row turn eight pairs each with the sines of
-// their eight pairs in registers for every row they visit, the next row's loads in flight.
+// their eight pairs in registers for every row they visit, the next row's loads in flight as they come (converted
+// on arrival they held up the row before: 6000 tokens of 32 + 8 + 8 f16 heads of 128 to E4M3 with their read 78 us, now 63;
+// two rows ahead 68).
 // Measured: 8192 tokens of 64 + 8 + 8 f32 heads of 64, 252 MB: 48 us, 5.2 TB/s, 0.80 of the copy bandwidth.
 //
 // E4M3 rows: the scale is a power of two, so scaling is exact and only the rounding to E4M3
@@ -21,7 +23,7 @@ namespace amoe {
 namespace attn {
 namespace {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendWarps = 4;  // of a CTA, at most
 constexpr int kReadThreads = 256;
 constexpr int kReadTokens = 4;  // rows of a warp
 constexpr int kNoRow = INT_MIN;  // in the place of a page: not a row of this call
@@ -36,7 +38,7 @@ struct AppendParams {
     CacheDev c;
     RowsDev q, k, v, q_out, k_out, v_out;
     const int32_t *cu, *past;
-    int tokens, seqs, q_heads, q_out_type, k_out_type, v_out_type, warps;  // warps to a token
+    int tokens, seqs, q_heads, q_out_type, k_out_type, v_out_type;
     RopeDev rope;
 };
 
@@ -105,20 +107,16 @@ __device__ __forceinline__ void cache_store(char *pages, uint8_t *scales, int64_
 }
 
 template <int D, int SRC, int CACHE>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int L = D / 16;  // lanes of a row
     constexpr int STEP = 32 / L;  // rows of a warp at a time
     constexpr int ES = SRC == AMOE_GGUF_F32 ? 4 : 2;
-    __shared__ double2 cs_all[kAppendThreads / 32][D / 2];
-    const int lane = threadIdx.x % 32, part = lane % L, warp = threadIdx.x / 32, mine = warp % p.warps;
-    double2 *cs = cs_all[warp / p.warps];  // one for each token of the CTA
-    const int64_t token = (int64_t)blockIdx.x * (kAppendThreads / 32 / p.warps) + warp / p.warps;
-    const bool given = token < p.tokens && token < p.cu[p.seqs];
-    const int t = given ? (int)token : 0, r0 = mine * STEP + lane / L;
-    const int rows = given ? p.q_heads + 2 * p.c.heads : 0;
+    __shared__ double2 cs[D / 2];
+    const int lane = threadIdx.x % 32, part = lane % L, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    const int t = blockIdx.x, r0 = warp * STEP + lane / L, rows = p.q_heads + 2 * p.c.heads;
 
-    struct Row {
-        float a[8], b[8];
+    struct Row {  // as loaded: a conversion would wait for it
+        uint4 a[ES / 2], b[ES / 2];
     };
     auto load = [&](int r, Row &x) {
         if (r >= rows) return;
@@ -126,29 +124,30 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         const RowsDev &src = is_q ? p.q : is_k ? p.k : p.v;
         const int h = is_q ? r : is_k ? r - p.q_heads : r - p.q_heads - p.c.heads;
         const char *at = src.p + t * src.ts + h * src.hs + part * 8 * ES;
-        load8<SRC>(at, x.a);
-        load8<SRC>(at + D / 2 * ES, x.b);
+#pragma unroll
+        for (int i = 0; i < ES / 2; ++i) {
+            x.a[i] = reinterpret_cast<const uint4 *>(at)[i];
+            x.b[i] = reinterpret_cast<const uint4 *>(at + D / 2 * ES)[i];
+        }
     };
     Row next{};
     load(r0, next);  // on its way while the position and its sines are found
 
-    int64_t pos = -1;
-    int page = -1;
-    if (given) {
-        int found[1];
-        find_seqs(p.cu, p.seqs, t, found);
-        const int s = found[0], start = p.cu[s], past = p.past[s];
-        if (start > t || start < 0 || p.cu[s + 1] <= t || past < 0) {
-            if (lane == 0) atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
-        } else {
-            pos = (int64_t)past + (t - start);
-            page = page_of(p.c, s, pos);
-        }
+    const int last = p.cu[p.seqs];
+    int found[1];
+    find_seqs(p.cu, p.seqs, t, found);
+    const int s = found[0], start = p.cu[s], past = p.past[s];
+    if (t >= last) return;  // rows behind the last sequence
+    if (start > t || start < 0 || p.cu[s + 1] <= t || past < 0) {
+        if (threadIdx.x == 0) atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
+        return;
     }
+    const int64_t pos = (int64_t)past + (t - start);
+    const int page = page_of(p.c, s, pos);
     double2 w[8];
     if (p.rope.on) {
         // the token's warps share its sines
-        for (int i = mine * 32 + lane; i < D / 2; i += 32 * p.warps) {
+        for (int i = threadIdx.x; i < D / 2; i += blockDim.x) {
             double sn, c;
             sincos((double)pos * p.rope.freq[i], &sn, &c);
             cs[i] = make_double2(c * p.rope.conc, sn * p.rope.conc);
@@ -157,12 +156,14 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = cs[part * 8 + i];
     }
-    if (pos < 0) return;
-
     // the warp stays together for the row maximum's shuffles: the bound is the warp's first row
-    for (int r = r0; r - lane / L < rows; r += STEP * p.warps) {
-        Row x = next;
-        load(r + STEP * p.warps, next);
+    for (int r = r0; r - lane / L < rows; r += STEP * warps) {
+        struct {
+            float a[8], b[8];
+        } x;
+        load8<SRC>(reinterpret_cast<const char *>(next.a), x.a);
+        load8<SRC>(reinterpret_cast<const char *>(next.b), x.b);
+        load(r + STEP * warps, next);
         const bool live = r < rows;
         const bool is_q = r < p.q_heads, is_k = !is_q && r < p.q_heads + p.c.heads;
         const int h = is_q ? r : is_k ? r - p.q_heads : r - p.q_heads - p.c.heads;
@@ -281,10 +282,12 @@ __global__ void __launch_bounds__(kReadThreads, 4) read_kernel(const __grid_cons
 
 template <int D, int SRC>
 cudaError_t launch_append(const AppendParams &p, int cache, cudaStream_t st) {
-    const int grid = (p.tokens - 1) / (kAppendThreads / 32 / p.warps) + 1;
-    if (cache == AMOE_GGUF_F16) append_kernel<D, SRC, AMOE_GGUF_F16><<<grid, kAppendThreads, 0, st>>>(p);
-    else if (cache == AMOE_GGUF_BF16) append_kernel<D, SRC, AMOE_GGUF_BF16><<<grid, kAppendThreads, 0, st>>>(p);
-    else append_kernel<D, SRC, AMOE_KV_E4M3><<<grid, kAppendThreads, 0, st>>>(p);
+    // A CTA a token: one warp, or four where the tokens alone do not fill the GPU.  8192 tokens of 64-wide f32 heads: 47.9 us with one warp to a token, 51 with two, 61 with four; 6000 of 128-wide
+    // f16 ones with their read: 63.4, 68, 78.
+    const int grid = p.tokens, threads = p.tokens < 148 * 8 ? 32 * kAppendWarps : 32;
+    if (cache == AMOE_GGUF_F16) append_kernel<D, SRC, AMOE_GGUF_F16><<<grid, threads, 0, st>>>(p);
+    else if (cache == AMOE_GGUF_BF16) append_kernel<D, SRC, AMOE_GGUF_BF16><<<grid, threads, 0, st>>>(p);
+    else append_kernel<D, SRC, AMOE_KV_E4M3><<<grid, threads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -366,9 +369,6 @@ int amoe_kv_append(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const i
     p.q_out_type = q_out ? q_out->type : 0;
     p.k_out_type = k_out ? k_out->type : 0;
     p.v_out_type = v_out ? v_out->type : 0;
-    // Warps to a token: as many as its sines fill; four where the tokens alone do not fill the GPU.  8192 tokens of
-    // 64-wide heads: 48 us with one, 51 with two, 61 with four; 6000 of 128-wide ones: 79, 77.5, 86.
-    p.warps = tokens < 148 * 8 ? 4 : D / 64;
     if (rope) {
         for (int i = 0; i < D / 2; ++i) p.rope.freq[i] = rope->freq[i];
         p.rope.conc = rope->concentration;
