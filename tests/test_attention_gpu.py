@@ -822,3 +822,27 @@ def test_a_split_prefill_is_captured_and_sees_nothing(cuda_device):
         assert (out[:30 - seen] == 0).all()
         if seen:
             R.close(out[30 - seen:], *R.attention(q[30 - seen:].cpu(), k[:n].cpu(), v[:n].cpu()))
+
+
+def test_split_prefills_on_two_streams_and_strided_rows(cuda_device):
+    g = gen(311)
+    heads, kv, d, n, m = 16, 2, 64, 24, 7000
+    calls = []
+    for _ in range(2):
+        fused = randn(g, n, (heads + 2) * d, dtype=BF16).cuda()  # queries beside something else
+        q = fused[:, d:(heads + 1) * d].view(n, heads, d)
+        both = randn(g, m, 2, kv, d, dtype=BF16).cuda()  # keys and values of a token side by side
+        out = torch.full((n, heads, d + 8), 7.0, dtype=BF16, device="cuda")
+        calls.append((q, both[:, 0], both[:, 1], out))
+    cu_q, cu_k = i32([0, 9, n]).cuda(), i32([0, 4000, m]).cuda()
+    assert moe.load_library().amoe_attn_prefill_workspace(d, 0, heads, kv, n, m, 2) > 0
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (q, k, v, out) in zip(streams, calls):
+            attention.prefill(q, k, v, cu_q, cu_k, out=out[:, :, :d], stream=stream)
+    torch.cuda.synchronize()
+    for q, k, v, out in calls:
+        assert (out[:, :, d:] == 7).all()
+        for a, b, x, y in ((0, 9, 0, 4000), (9, n, 4000, m)):
+            R.close(out[a:b, :, :d], *R.attention(q[a:b].cpu(), k[x:y].cpu(), v[x:y].cpu()))
