@@ -20,7 +20,8 @@
 //     partial sums join through distributed shared memory: one launch.  A few long sequences
 //     need more CTAs than clusters can place (clusters of 16 left SMs idle: 59 us instead of 50 for
 //     131072 tokens of 8 f16 heads), so they write partial sums to the caller's workspace and
-//     a second kernel, whose launch overlaps the first, joins them.  No atomics: the order of addition
+//     a second kernel, whose launch overlaps the first, joins them.  So do a few sequences of lengths that
+//     may differ: the device shares the CTAs out by the lengths.  No atomics: the order of addition
 //     does not depend on timing.
 //
 // E4M3 keys and values meet f16 operands (every code is an f16 value).  A key's scale multiplies
@@ -56,7 +57,9 @@ struct DecodeParams {
     const float *sinks;
     float *work;  // partial sums of the CTAs, where they do not join in a cluster
     float scale_log2;
-    int window, group, q_type, split;
+    int window, group, q_type;
+    int split;  // CTAs to a (sequence, group of heads); where they join through work: to all sequences of a group of heads
+    int seqs;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
@@ -196,6 +199,56 @@ __device__ __forceinline__ void finish(const DecodeParams &p, int seq, int h, in
     store_row(p, seq, h, i % (D / 4), a, sum, top, y);
 }
 
+// The tiles of `keys` keys that a sequence's query sees, and the first one's first key.
+struct Seen {
+    int from, end, base, tiles;
+};
+__device__ __forceinline__ Seen seen_of(const DecodeParams &p, int len, int keys) {
+    Seen s;
+    const int64_t cap = (int64_t)p.c.table_stride << p.c.shift;
+    s.from = p.window > 0 && len > p.window ? len - p.window : 0;
+    s.end = len < cap ? len : (int)cap;
+    s.base = s.from / keys * keys;
+    s.tiles = s.end > s.from ? (s.end - s.base - 1) / keys + 1 : 0;
+    return s;
+}
+
+// CTAs first .. first + split - 1 of p.split take a sequence: one, and of the others a share like its tiles'.
+struct Share {
+    int seq, first, split;
+};
+// CTA x's share (seq < 0), or a sequence's.  Called by whole warps; split 0: the CTA has none.
+__device__ __forceinline__ Share share_of(const DecodeParams &p, int keys, int x, int seq) {
+    if (p.seqs == 1) return {0, 0, min(p.split, kMaxWide)};
+    const int lane = threadIdx.x % 32;
+    int64_t total = 0;
+    for (int s = lane; s < p.seqs; s += 32) total += seen_of(p, p.kv_len[s], keys).tiles;
+#pragma unroll
+    for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
+    int before = 0;
+    for (int s0 = 0; s0 < p.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < p.seqs)
+            n = 1 + (int)min((int64_t)kMaxWide - 1,
+                             seen_of(p, p.kv_len[s], keys).tiles * (int64_t)(p.split - p.seqs) / max(total, (int64_t)1));
+        int upto = n;
+#pragma unroll
+        for (int i = 1; i < 32; i <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, i);
+            if (lane >= i) upto += y;
+        }
+        const int first = before + upto - n;
+        const uint32_t hit = __ballot_sync(0xffffffffu, s < p.seqs && (seq < 0 ? x >= first && x < first + n : s == seq));
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            return {s0 + at, __shfl_sync(0xffffffffu, first, at), __shfl_sync(0xffffffffu, n, at)};
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {0, 0, 0};
+}
+
 template <int D, int CACHE, int NB, bool WIDE>
 __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && Tile<D, CACHE>::kCtas > 3)) decode_attn_kernel(const __grid_constant__ DecodeParams p) {
     using T = Tile<D, CACHE>;
@@ -204,7 +257,14 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
     extern __shared__ __align__(128) char smem[];
     namespace cg = cooperative_groups;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
-    const int split = p.split, rank = blockIdx.x, seq = blockIdx.z;
+    int split = p.split, rank = blockIdx.x, seq = blockIdx.z;
+    if constexpr (WIDE) {
+        cudaTriggerProgrammaticLaunchCompletion();
+        const Share share = share_of(p, KEYS, rank, -1);
+        if (share.split == 0) return;
+        split = share.split, seq = share.seq, rank -= share.first;
+        if (rank >= split) return;
+    }
     const int kvh = blockIdx.y % p.c.heads, row0 = blockIdx.y / p.c.heads * 16;
     char *ring = smem + warp * ((T::kWarpBytes + 127) / 128 * 128);
     uint32_t *side = reinterpret_cast<uint32_t *>(ring + STAGES * T::kStage);  // [STAGES][2][32] scale words, then masks
@@ -212,15 +272,12 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
     const uint32_t ring_a = smem_addr(ring);
 
     const int len = p.kv_len[seq];
-    const int from = p.window > 0 && len > p.window ? len - p.window : 0;
-    const int64_t cap = (int64_t)p.c.table_stride << p.c.shift;
-    const int end = len < cap ? len : (int)cap;
+    const Seen seen = seen_of(p, len, KEYS);
+    const int from = seen.from, end = seen.end, base = seen.base, ntile = seen.tiles;
     if (threadIdx.x == 0 && rank == 0) {
         if (len < 0) atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
-        if (len > cap) atomicOr(p.c.status, AMOE_KV_PAST_TABLE);
+        if (len > end) atomicOr(p.c.status, AMOE_KV_PAST_TABLE);
     }
-    const int base = from / KEYS * KEYS;
-    const int ntile = end > from ? (end - base - 1) / KEYS + 1 : 0;
     const int t0 = (int)((int64_t)ntile * rank / split) + warp, t1 = (int)((int64_t)ntile * (rank + 1) / split);
 
     // The queries of NB blocks of eight heads as the scores' B operand: lane's head g of a block.  qs: the factors of the
@@ -585,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
     if constexpr (WIDE) {
         __syncthreads();
         float4 *dst = reinterpret_cast<float4 *>(
-            p.work + (((int64_t)seq * gridDim.y + blockIdx.y) * split + rank) * T::kPart);
+            p.work + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * T::kPart);
         for (int i = threadIdx.x; i < T::kPart / 4; i += kThreads)
             if (i < LIVE * D / 4 || i >= 4 * D) dst[i] = reinterpret_cast<const float4 *>(part)[i];
         return;
@@ -613,12 +670,14 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     __shared__ float4 acc[LANES][COLS];
     const int seq = blockIdx.z, kvh = blockIdx.y % p.c.heads, row0 = blockIdx.y / p.c.heads * 16, r = blockIdx.x;
     if (row0 + r >= p.group) return;
+    const Share share = share_of(p, T::kKeys, 0, seq);
+    const int split = share.split;
     cudaGridDependencySynchronize();  // launched while the partial sums are still being made
     const int h = kvh * p.group + row0 + r, tid = threadIdx.x;
-    const float *work = p.work + ((int64_t)seq * gridDim.y + blockIdx.y) * p.split * T::kPart;
+    const float *work = p.work + ((int64_t)blockIdx.y * p.split + share.first) * T::kPart;
     const float sink = p.sinks ? p.sinks[h] * kLog2e : -INFINITY;
     float m = -INFINITY, n = -INFINITY, l = 0.0f;
-    if (tid < p.split) {
+    if (tid < split) {
         const float *x = work + (int64_t)tid * T::kPart + 16 * D + r;
         m = x[0], n = x[16], l = x[32];
     }
@@ -638,12 +697,12 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
 #pragma unroll
     for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
     if (tid % 32 == 0) total[tid / 32] = sum;
-    if (tid < p.split) factor[tid] = exp2f(m - z);
+    if (tid < split) factor[tid] = exp2f(m - z);
     __syncthreads();
     const int col = tid % COLS, lane = tid / COLS;
     float4 a = make_float4(0, 0, 0, 0);
 #pragma unroll 4
-    for (int w = lane; w < p.split; w += LANES) {
+    for (int w = lane; w < split; w += LANES) {
         const float f = factor[w];
         const float4 v = *reinterpret_cast<const float4 *>(work + (int64_t)w * T::kPart + r * D + col * 4);
         a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
@@ -675,7 +734,7 @@ cudaError_t launch(const DecodeParams &p, int device, int units, int seqs, cudaS
         ready[device].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.split, units, seqs);
+    cfg.gridDim = dim3(p.split, units, WIDE ? 1 : seqs);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = T::kSmem;
     cfg.stream = st;
@@ -705,19 +764,23 @@ struct Layout {
     int64_t bytes;
 };
 
-// Clusters (powers of two up to kCluster) while they fill the GPU: one launch.  Where even the largest
-// leaves it half empty and the length allows more, as many CTAs as fit at once, joined by a second launch.
+// Clusters (powers of two up to kCluster) while they fill the GPU: one launch.  Where even the largest leaves it half empty
+// and the length allows more, or where the lengths may differ much and there are CTAs enough to share them out finely, as
+// many CTAs as fit at once, joined by a second launch.  Cluster -> shared, 8 kv heads of 64: 7 sequences of 500-2000
+// tokens and one of 60000, bf16, 58 -> 29 us, E4M3 60 -> 25; 8 of 10000-20000 46 -> 43 and 36 -> 32; 8 of 20000 62 -> 55 and
+// 38 -> 38; 4 of 20000 29 -> 32 and 26 -> 24.  With fewer than four CTAs a sequence it loses: 32 of 8192, bf16, 87 -> 92,
+// 48 of 4096-8192, E4M3, 71 -> 94; and so it does for short ones: 8 of 700, E4M3, 7.6 -> 9.3.
 Layout layout(int64_t units, int64_t seqs, int64_t tokens, int row_bytes, int part_floats, int ctas) {
     const int keys = row_bytes == 256 ? 16 : 32;
     const int64_t tiles = (tokens - 1) / keys + 1, all = units * seqs;
     const int want = 6 * 148;
     Layout l{1, false, 0};
     while (l.split < kCluster && all * l.split < want && tiles > l.split * kWarps) l.split *= 2;
-    if (l.split == kCluster && all * l.split < want / 2) {
-        const int64_t fit = ctas * 148 / all, most = tiles / kWarps;
-        const int64_t s = std::min<int64_t>({fit, most, kMaxWide});
-        if (s > l.split) l = {(int)s, true, all * s * part_floats * 4};
-    }
+    const int64_t fit = std::min<int64_t>(ctas * 148 / units, kMaxWide * seqs);
+    const int64_t s = std::min<int64_t>(fit, tiles * seqs / kWarps);
+    const bool idle = l.split == kCluster && all * l.split < want / 2 && s > l.split * seqs;
+    const bool shared = seqs > 1 && fit >= 4 * seqs && tokens >= 8192;
+    if (idle || shared) l = {(int)s, true, units * s * part_floats * 4};
     return l;
 }
 
@@ -807,7 +870,7 @@ int amoe_attn_decode(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const
     if (l.wide && (!workspace || workspace_bytes < l.bytes))
         return reject("decode needs a workspace of " + std::to_string(l.bytes) + " bytes");
     if (l.wide && (reinterpret_cast<uintptr_t>(workspace) & 15)) return reject("workspace must be 16-byte aligned");
-    p.split = l.split, p.work = static_cast<float *>(workspace);
+    p.split = l.split, p.seqs = seqs->seqs, p.work = static_cast<float *>(workspace);
     DeviceScope scope;
     cudaError_t e = scope.enter(cache->device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");

@@ -439,7 +439,8 @@ AMOE_API int amoe_attn_decode(const amoe_kv_cache *cache, const amoe_kv_seqs *se
                               void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Bytes of workspace that amoe_attn_decode needs for these shapes (the cache's and seqs'
- * device memory is not looked at; no GPU needed), 0 where one launch does; negative: an error. */
+ * device memory is not looked at; no GPU needed), 0 where one launch does; negative: an error.
+ * Long sequences need one, up to a few to the GPU. */
 AMOE_API int64_t amoe_attn_decode_workspace(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, int32_t q_heads,
                                             int32_t window, int32_t max_len);
 

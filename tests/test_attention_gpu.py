@@ -846,3 +846,59 @@ def test_split_prefills_on_two_streams_and_strided_rows(cuda_device):
         assert (out[:, :, d:] == 7).all()
         for a, b, x, y in ((0, 9, 0, 4000), (9, n, 4000, m)):
             R.close(out[a:b, :, :d], *R.attention(q[a:b].cpu(), k[x:y].cpu(), v[x:y].cpu()))
+
+
+SHARES = [  # lengths of one call that the device shares the CTAs out by, heads, kv_heads, d, page, cache, window, sinks
+    ([9000, 1, 0, 300, 8191, 77], 8, 1, 64, 64, BF16, 0, True),
+    ([17, 12001], 8, 2, 128, 16, E4M3, 0, True),
+    ([0, 0, 10000], 16, 1, 64, 128, F16, 0, False),
+    ([9999, 20000, 8200], 8, 1, 64, 32, E4M3, 8500, False),
+    ([8300] + [5] * 69, 16, 1, 64, 64, BF16, 0, True),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SHARES)))
+def test_decode_of_uneven_lengths(cuda_device, case):
+    lens, heads, kv, d, page, kind, window, with_sinks = SHARES[case]
+    g = gen(400 + case)
+    table, pool = table_for(g, lens, page)
+    pages = filled(g, pool, kv, page, d, kind)
+    q = randn(g, len(lens), heads, d, dtype=BF16 if kind == E4M3 else kind, scale=2.0)
+    sinks = randn(g, heads, scale=2.0) if with_sinks else None
+    cache = on_gpu(pages)
+    length, dq, dt = i32(lens).cuda(), q.cuda(), table.cuda()
+    want = []
+    for i, n in enumerate(lens):
+        zero = torch.zeros(1, heads, d, dtype=torch.float64)
+        want.append(R.attention(q[i:i + 1], *(R.rows_of(c, s, table[i], 0, n) for c, s in pages), sinks, window)
+                    if n else (zero, zero))
+    kw = dict(window=window, sinks=None if sinks is None else sinks.cuda())
+    out = cache.decode(dq, dt, length, **kw)
+    assert max(cache._workspace.values()) > 0
+    cache.check()
+    for i, w in enumerate(want):
+        R.close(out[i:i + 1], *w)
+    # captured; then other lengths in the same graph: all zero, one of them negative, one beyond the table
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.decode(dq, dt, length, **kw)
+    graph.replay()
+    for i, w in enumerate(want):
+        R.close(out[i:i + 1], *w)
+    length.zero_()
+    graph.replay()
+    assert (out == 0).all()
+    cache.check()
+    length[0] = -5
+    graph.replay()
+    assert (out == 0).all()
+    with pytest.raises(AmoeError):
+        cache.check()
+    length[0] = 1 << 30
+    graph.replay()
+    with pytest.raises(AmoeError):
+        cache.check()
+    length.copy_(i32(lens))
+    graph.replay()
+    for i, w in enumerate(want):
+        R.close(out[i:i + 1], *w)
