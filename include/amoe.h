@@ -440,7 +440,7 @@ AMOE_API int amoe_attn_decode(const amoe_kv_cache *cache, const amoe_kv_seqs *se
 
 /* Bytes of workspace that amoe_attn_decode needs for these shapes (the cache's and seqs'
  * device memory is not looked at; no GPU needed), 0 where one launch does; negative: an error.
- * Long sequences need one, up to a few to the GPU. */
+ * Calls of a few sequences, one of which may be long, need one. */
 AMOE_API int64_t amoe_attn_decode_workspace(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, int32_t q_heads,
                                             int32_t window, int32_t max_len);
 
