@@ -726,6 +726,7 @@ Layout layout(int head_dim, int window, int64_t q_tokens, int64_t k_tokens, int6
     const int64_t slots = kSms * (head_dim == 64 ? Cfg<64>::kCtas : Cfg<128>::kCtas);
     const int64_t whole = tiles / slots * slots, rest = tiles - whole;
     Layout l{tiles, tiles, 1, 0};
+    if (rest == 0) return l;  // whole waves (or no rows): nothing to split
     // The host knows no sequence's own length and takes them as equal.  A sequence's first tokens come last and
     // see the fewest keys.
     const int64_t most = window > 0 ? (int64_t)window + tile_tokens : INT_MAX, keys = k_tokens / seqs;
