@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(kReadThreads, 4) read_kernel(const __grid_cons
         const int64_t f = p.first ? p.first[s] : 0;
         if (start < 0 || start > t || p.cu[s + 1] <= t || f < 0) {
             atomicOr(p.c.status, AMOE_KV_BAD_LENGTHS);
+            page = -AMOE_KV_BAD_LENGTHS;  // a row of this call all the same: zeros
         } else {
             pos = f + (t - start);
             page = page_of(p.c, s, pos);

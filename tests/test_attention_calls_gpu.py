@@ -26,3 +26,31 @@ def test_prefill_of_whole_waves(cuda_device, n, before, heads, kv, d):
         want, bound = R.attention(q[:, h:h + 1], k[:, one:one + 1], v[:, one:one + 1])
         R.close(out[:, h:h + 1], want, bound)
     assert torch.isfinite(out).all()
+
+
+# ---- wrong lengths -----------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,out", [(BF16, BF16), (E4M3, F32)])
+def test_read_of_wrong_lengths_gives_zeros(cuda_device, kind, out):
+    """Rows below cu[seqs] whose start or first position is wrong are zeros, not what the output held; the others are read."""
+    g = gen(61)
+    kv, d, page = 3, 64, 16
+    table, pool = table_for(g, [40, 40], page)
+    pages = filled(g, pool, kv, page, d, kind)
+    cache = on_gpu(pages)
+    held = [[R.rows_of(c, s, table[i], 0, 40).to(out) for c, s in pages] for i in range(2)]
+    for cu, first, rows in [  # rows: (sequence, its position) of each output row, None: zeros
+        ([0, 10, 14], [-1, 2], [None] * 10 + [(1, 2 + i) for i in range(4)]),
+        ([0, 10, 14], [3, -(1 << 31)], [(0, 3 + i) for i in range(10)] + [None] * 4),
+        ([3, 9, 9], [0, 0], [None] * 3 + [(0, i) for i in range(6)]),
+        ([-2, 4, 6], [0, 0], [None] * 4 + [(1, 0), (1, 1)]),
+    ]:
+        k = torch.full((20, kv, d), 7.0, dtype=out, device="cuda")
+        v = torch.full((20, kv, d), 7.0, dtype=out, device="cuda")
+        cache.read(table.cuda(), i32(cu).cuda(), 20, first=i32(first).cuda(), k_out=k, v_out=v)
+        with pytest.raises(AmoeError, match="lengths"):
+            cache.check()
+        for got, which in ((k.cpu(), 0), (v.cpu(), 1)):
+            for t, at in enumerate(rows):
+                want = torch.zeros(kv, d, dtype=out) if at is None else held[at[0]][which][at[1]]
+                assert torch.equal(got[t], want), (cu, first, t)
+            assert (got[len(rows):] == 7).all()
