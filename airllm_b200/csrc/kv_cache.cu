@@ -42,6 +42,17 @@ struct AppendParams {
     RopeDev rope;
 };
 
+// Starts that are negative, decrease or pass the rows given leave rows that no CTA looks at, or that it takes for rows
+// behind the last sequence.  The grid's last CTA, which has no row, looks at all of them.
+__device__ __forceinline__ void check_starts(const int32_t *cu, int seqs, int tokens, int32_t *status) {
+    bool bad = false;
+    for (int s = threadIdx.x; s < seqs; s += blockDim.x) {
+        const int a = cu[s], b = cu[s + 1];
+        bad |= a < 0 || b < a || b > tokens;
+    }
+    if (bad) atomicOr(status, AMOE_KV_BAD_LENGTHS);
+}
+
 // Smallest e with amax <= 448 * 2^e, at least -127; 0 for amax == 0.  amax = 1.f * 2^(E - 127)
 // and 448 * 2^e = 1.75 * 2^(e + 8).
 __device__ __forceinline__ int e4m3_exp(float amax) {
@@ -113,6 +124,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const __grid_
     constexpr int ES = SRC == AMOE_GGUF_F32 ? 4 : 2;
     __shared__ double2 cs[D / 2];
     const int lane = threadIdx.x % 32, part = lane % L, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    if (blockIdx.x == gridDim.x - 1) return check_starts(p.cu, p.seqs, p.tokens, p.c.status);
     const int t = blockIdx.x, r0 = warp * STEP + lane / L, rows = p.q_heads + 2 * p.c.heads;
 
     struct Row {  // as loaded: a conversion would wait for it
@@ -204,6 +216,7 @@ template <int D, int CACHE>
 __global__ void __launch_bounds__(kReadThreads, 4) read_kernel(const __grid_constant__ ReadParams p) {
     constexpr int E = CACHE == AMOE_KV_E4M3 ? 16 : 8;  // elements of 16 bytes
     constexpr int C = D / E, RPI = 32 / C, BATCH = 4;  // lanes of a row, rows at a time, batches of them
+    if (blockIdx.x == gridDim.x - 1) return check_starts(p.cu, p.seqs, p.tokens, p.c.status);
     const int lane = threadIdx.x % 32, ch = lane % C;
     const int64_t first_row = ((int64_t)blockIdx.x * (kReadThreads / 32) + threadIdx.x / 32) * kReadTokens;
     const int last = min(p.cu[p.seqs], p.tokens);
@@ -283,9 +296,9 @@ __global__ void __launch_bounds__(kReadThreads, 4) read_kernel(const __grid_cons
 
 template <int D, int SRC>
 cudaError_t launch_append(const AppendParams &p, int cache, cudaStream_t st) {
-    // A CTA a token: one warp, or four where the tokens alone do not fill the GPU.  8192 tokens of 64-wide f32 heads: 47.9 us with one warp to a token, 51 with two, 61 with four; 6000 of 128-wide
+    // A CTA a token, and one for the starts: one warp, or four where the tokens alone do not fill the GPU.  8192 tokens of 64-wide f32 heads: 47.9 us with one warp to a token, 51 with two, 61 with four; 6000 of 128-wide
     // f16 ones with their read: 63.4, 68, 78.
-    const int grid = p.tokens, threads = p.tokens < 148 * 8 ? 32 * kAppendWarps : 32;
+    const int grid = p.tokens + 1, threads = p.tokens < 148 * 8 ? 32 * kAppendWarps : 32;
     if (cache == AMOE_GGUF_F16) append_kernel<D, SRC, AMOE_GGUF_F16><<<grid, threads, 0, st>>>(p);
     else if (cache == AMOE_GGUF_BF16) append_kernel<D, SRC, AMOE_GGUF_BF16><<<grid, threads, 0, st>>>(p);
     else append_kernel<D, SRC, AMOE_KV_E4M3><<<grid, threads, 0, st>>>(p);
@@ -301,7 +314,7 @@ cudaError_t launch_append_d(const AppendParams &p, int src, int cache, cudaStrea
 
 template <int D>
 cudaError_t launch_read_d(const ReadParams &p, int cache, cudaStream_t st) {
-    const int grid = (p.tokens - 1) / (kReadTokens * kReadThreads / 32) + 1;
+    const int grid = (p.tokens - 1) / (kReadTokens * kReadThreads / 32) + 2;
     if (cache == AMOE_GGUF_F16) read_kernel<D, AMOE_GGUF_F16><<<grid, kReadThreads, 0, st>>>(p);
     else if (cache == AMOE_GGUF_BF16) read_kernel<D, AMOE_GGUF_BF16><<<grid, kReadThreads, 0, st>>>(p);
     else read_kernel<D, AMOE_KV_E4M3><<<grid, kReadThreads, 0, st>>>(p);
@@ -346,6 +359,7 @@ int amoe_kv_append(const amoe_kv_cache *cache, const amoe_kv_seqs *seqs, const i
     if (int rc = check_cache(cache, seqs)) return rc;
     if (!cu || !past) return reject("cu and past must not be NULL");
     if (tokens < 0) return reject("tokens must not be negative");
+    if (tokens == INT_MAX) return reject("more than 2^31 - 2 tokens in one append call");  // a CTA each, and one more
     const int D = cache->head_dim, kv = cache->kv_heads;
     if (int rc = check_rows(k, "k", D, kv, tokens, -1)) return rc;
     if (int rc = check_rows(v, "v", D, kv, tokens, k->type)) return rc;

@@ -43,3 +43,13 @@ def test_prefill_takes_the_workspace_that_it_asks_for(d, heads, kv):
                                            None, 0, None)
                 assert rc == moe.AMOE_ERR_CUDA, (behind, seqs, n, last_error())
     assert asked > 0
+
+
+def test_append_of_more_tokens_than_a_grid_holds():
+    lib, r = moe.load_library(), rows()
+    c = moe.AmoeKvCache(AT, AT, None, None, AT, 4, 16, 8, 64, BF16, 0)
+    s = moe.AmoeKvSeqs(AT, 4, 2)
+    flat = rows(ts=0)
+    assert lib.amoe_kv_append(ref(c), ref(s), AT, AT, 2 ** 31 - 1, None, None, ref(flat), ref(flat), None, None, None,
+                              None) == moe.AMOE_ERR_INVALID
+    assert "tokens" in last_error()

@@ -54,3 +54,38 @@ def test_read_of_wrong_lengths_gives_zeros(cuda_device, kind, out):
                 want = torch.zeros(kv, d, dtype=out) if at is None else held[at[0]][which][at[1]]
                 assert torch.equal(got[t], want), (cu, first, t)
             assert (got[len(rows):] == 7).all()
+
+
+def test_starts_that_decrease_or_pass_the_rows_are_reported(cuda_device):
+    g = gen(62)
+    kv, d, page, n = 2, 64, 16, 6
+    cache = attention.KVCache(8, page, kv, d, dtype=F16)
+    table = i32([[0, 1], [2, 3], [4, 5]]).cuda()
+    rows = randn(g, n, kv, d, dtype=F16).cuda()
+    zero = i32([0, 0, 0]).cuda()
+    for cu in ([0, 2, 4, 7], [0, 2, 4, 2 ** 31 - 1], [0, 5, 3, 3], [0, 5, 2, 6], [0, 2, 9, 6], [0, -3, 4, 6]):
+        cache.append(rows, rows, table, zero, i32(cu).cuda())
+        with pytest.raises(AmoeError, match="lengths"):
+            cache.check()
+        cache.read(table, i32(cu).cuda(), n)
+        with pytest.raises(AmoeError, match="lengths"):
+            cache.check()
+    # the rows that were given are there all the same, and fewer rows than were given are no mistake
+    cache.append(rows, rows, table, zero, i32([0, 2, 4, 9]).cuda())
+    with pytest.raises(AmoeError, match="lengths"):
+        cache.check()
+    k, v = cache.read(table, i32([0, 2, 4, 6]).cuda(), n)
+    assert torch.equal(k, rows) and torch.equal(v, rows)
+    cache.append(rows, rows, table, zero, i32([0, 2, 2, 5]).cuda())
+    cache.read(table, i32([0, 0, 0, 0]).cuda(), n)
+    cache.check()
+    # the last of many sequences
+    many = 3000
+    wide = torch.zeros(many, 2, dtype=torch.int32).cuda()
+    cu = torch.zeros(many + 1, dtype=torch.int32)
+    for at, bad in ((many, n + 1), (many - 1, n), (many - 1, 1)):
+        cu.zero_()
+        cu[at] = bad
+        cache.append(rows, rows, wide, torch.zeros(many, dtype=torch.int32).cuda(), cu.cuda())
+        with pytest.raises(AmoeError, match="lengths"):
+            cache.check()
