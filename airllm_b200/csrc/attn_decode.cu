@@ -15,7 +15,7 @@
 //     never reaches the products.  A tile that lies in one page is copied as one run; smaller pages
 //     have each lane look up its key;
 //   - a head's running maximum is lazy: it moves, and the sums are rescaled, when some weight has outgrown it by
-//     2^8, which one vote a tile finds out;
+//     2^8 (2^4 in f16, whose weights carry a factor: attn.cuh), which one vote a tile finds out;
 //   - the keys of one (sequence, kv head) are split over the CTAs of a cluster of up to 8, whose
 //     partial sums join through distributed shared memory: one launch.  A few long sequences
 //     need more CTAs than clusters can place (clusters of 16 left SMs idle: 59 us instead of 50 for
@@ -46,7 +46,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kLazy = 8.0f;  // log2 growth of a head's maximum that is left in the weights
 constexpr int kCluster = 8;
 constexpr int kMaxWide = 256;  // CTAs that the join kernel takes: one for each of its threads
 
@@ -143,6 +142,8 @@ template <int D, int CACHE>
 struct Tile {
     static constexpr bool kFp8 = CACHE == AMOE_KV_E4M3;
     static constexpr int kType = kFp8 ? AMOE_GGUF_F16 : CACHE;
+    static constexpr float kShift = weight_shift(kType);        // log2 of the weights' factor
+    static constexpr float kTop = kShift + weight_lazy(kType);  // and of the largest weight
     static constexpr int kRow = D * (kFp8 ? 1 : 2);             // bytes of a cache row
     static constexpr int kKeys = kRow == 256 ? 16 : 32;         // keys of a warp's tile
     static constexpr int kStage = 2 * kKeys * kRow;             // K then V
@@ -398,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
         if (lane == 0) masks[stage] = live;
     };
 
-    // o: rows are elements, columns heads; m, n, l: of the lane's two heads of each block, l over its own keys
+    // o: rows are elements, columns heads; m, n, l: of the lane's two heads of each block, l over its own keys.  m: the
+    // maximum less kShift, which o (and l, but for E4M3) is relative to; n: the maximum that l is relative to for E4M3
     float o[D / 16][NB][4] = {}, m[NB][2], n[NB][2], l[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -497,11 +499,12 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
                     for (int i = 0; i < 2; ++i) {
                         float &x = sc[t16][nb][2 * hi + i];
                         x = on ? x * (T::kFp8 ? by * qs[nb][i] : qs[nb][i]) : -INFINITY;
-                        if constexpr (T::kFp8) grown |= x - n[nb][i] > kLazy;
-                        grown |= x + ev[t16][hi] - m[nb][i] > kLazy;
+                        if constexpr (T::kFp8) grown |= x - n[nb][i] > 8.0f;
+                        grown |= x + ev[t16][hi] - m[nb][i] > T::kTop;
                     }
             }
-        // The maxima are lazy: they move, and what hangs on them with them, when some weight outgrew its own by 2^8.
+        // The maxima are lazy: they move, and what hangs on them with them, when some weight outgrew
+        // what it may (2^15 in f16, 2^8 in bf16 and in E4M3's denominator).
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
                             top = fmaxf(top, sc[t16][nb][2 * hi + i] + ev[t16][hi]);
                             ntop = fmaxf(ntop, sc[t16][nb][2 * hi + i]);
                         }
-                    const float mm = fmaxf(m[nb][i], keys_max(top)), keep = ex2(m[nb][i] - (mm == -INFINITY ? 0.0f : mm));
+                    const float mm = fmaxf(m[nb][i], keys_max(top) - T::kShift), keep = ex2(m[nb][i] - (mm == -INFINITY ? 0.0f : mm));
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) o[j][nb][i] *= keep, o[j][nb][2 + i] *= keep;
                     m[nb][i] = mm;

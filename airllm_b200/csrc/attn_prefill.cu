@@ -26,7 +26,8 @@
 // split over CTAs, and a second kernel joins the partial sums (`layout` below chooses, with what it measured).
 //
 // The maximum is lazy: O and the sum are rescaled only when a row's maximum has grown by more
-// than 2^8 since the last time, which float32 sums and 16-bit weights (relative precision) hold without loss.
+// than 2^8 since the last time, which float32 sums hold without loss.  Weights are 2^(score - maximum) in bf16, and 2^7
+// times that in f16 (attn.cuh: weight_shift).
 //
 // A key that a row must not see has weight 0, but 0 times an infinity or NaN in its value is NaN.
 // Values behind the tile's last visible key are overwritten with zeros in shared memory; a row whose
@@ -50,7 +51,6 @@ using bs::tc_fence_before;
 
 constexpr int kRows = 128;
 constexpr int kSoftWarps = 4, kFeedWarp = 4, kThreads = 160;
-constexpr float kLazy = 8.0f;  // log2 growth of a row's maximum that is left in the weights
 
 struct PrefillParams {
     RowsDev q, k, v, out;  // K and V for the rows that are computed again
@@ -278,7 +278,7 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, int par
     return false;
 }
 
-// A sink's share of the denominator beside the maximum z (in log2).  It may pass float32's range, and the row is then 0;
+// A sink's share of a denominator whose weights are relative to z (in log2).  It may pass float32's range, and the row is then 0;
 // a sink of +inf leaves inf / inf.
 __device__ __forceinline__ float sink_weight(float sink, float z) {
     return sink == INFINITY ? NAN : ex2(sink * kLog2e - z);
@@ -477,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         const int r = threadIdx.x, tok = r / p.group, head = kvh * p.group + r % p.group, at = at0 + tok;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+        constexpr float SHIFT = weight_shift(TYPE);  // O and l carry the weights' factor
         float m = -INFINITY, l = 0.0f;
         bool ok = true;  // after a wait that gave up the warp goes on to the end on what is there, and writes NaN
         for (int j = 0; j < tiles; ++j) {
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
             for (int i = 0; i < N; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             bool waited = j == 0;  // P and O are free once the products of the tile before are done
-            if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > kLazy)) {
+            if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > weight_lazy(TYPE))) {
                 const float mm = fmaxf(m, top);
                 if (j > 0) {
                     ok &= wait_warp(o_done, (uint32_t)(j - 1) & 1u, work);
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                 }
                 m = mm;
             }
-            const float off = m == -INFINITY ? 0.0f : m * p.scale_log2;
+            const float off = m == -INFINITY ? 0.0f : m * p.scale_log2 - SHIFT;
             const uint64_t off2 = pair(-off, -off);
             uint64_t sums[2] = {0, 0};
 #pragma unroll
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         if (SPLIT && part >= 0) {  // the row's sums over this part, for the kernel that joins them
             float *sums = p.work + (int64_t)((tile - p.whole) * p.split + part) * (D + 2) * kRows + r;
             if (mine) {
-                sums[D * kRows] = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+                sums[D * kRows] = m == -INFINITY ? -INFINITY : m * p.scale_log2 - SHIFT;
                 sums[(D + 1) * kRows] = ok ? l : NAN;
             }
 #pragma unroll
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                     if (mine) sums[(c + i) * kRows] = tiles > 0 ? o[i] : 0.0f;
             }
         } else {
-            if (p.sinks && mine) l += sink_weight(p.sinks[head], m == -INFINITY ? 0.0f : m * p.scale_log2);
+            if (p.sinks && mine) l += sink_weight(p.sinks[head], m == -INFINITY ? 0.0f : m * p.scale_log2 - SHIFT);
             // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
             const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
             char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;

@@ -89,3 +89,50 @@ def test_starts_that_decrease_or_pass_the_rows_are_reported(cuda_device):
         cache.append(rows, rows, wide, torch.zeros(many, dtype=torch.int32).cuda(), cu.cuda())
         with pytest.raises(AmoeError, match="lengths"):
             cache.check()
+
+
+# ---- weights of 16 bits ------------------------------------------------------------------------
+def tail(n, kv, d, t):
+    """(q row, k, v): one key of weight 1 with a zero value, then n - 1 keys of weight 2^-t with values of 1000."""
+    q = torch.zeros(d, dtype=F16)
+    k, v = torch.zeros(n, kv, d, dtype=F16), torch.full((n, kv, d), 1000.0, dtype=F16)
+    q[0], k[0, :, 0], v[0] = 1.0, t * math.log(2), 0.0
+    return q, k, v
+
+
+# What f16 weights lose beside attention_ref's bound: below 2^-25 of the row's largest weight (here 1, and the
+# denominator at least 1) half a step of the factor 2^11's subnormals, 2^-25 / 2^11, a key, times its value.
+def tail_bound(n):
+    return n * 2.0 ** -36 * 1000.0
+
+
+TAILS = [10.0, 20.3, 23.4, 24.9, 25.1, 27.0]
+
+
+@pytest.mark.parametrize("t", TAILS)
+@pytest.mark.parametrize("kind,n,kv", [(F16, 131072, 1), (F16, 4000, 2), (E4M3, 131072, 1), (E4M3, 4000, 2)])
+def test_decode_of_a_flat_tail(cuda_device, t, kind, n, kv):
+    d, page = 64, 128
+    q, k, v = tail(n, kv, d, t)
+    pages = -(-n // page)
+    cache = attention.KVCache(pages, page, kv, d, dtype=kind)
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    cache.append(k.cuda(), v.cuda(), table.cuda(), i32([0]).cuda(), i32([0, n]).cuda())
+    qs = q.expand(1, 4 * kv, d).contiguous()
+    got = cache.decode(qs.cuda(), table.cuda(), i32([n]).cuda(), scale=1.0)
+    held = (R.values(*R.e4m3(x.float())) for x in (k, v)) if kind == E4M3 else (k, v)
+    want, bound = R.attention(qs, *held, scale=1.0)
+    R.close(got, want, bound + tail_bound(n))
+
+
+@pytest.mark.parametrize("t", TAILS)
+@pytest.mark.parametrize("queries,n,heads,split", [(1, 131072, 2, True), (444, 6444, 128, False)])
+def test_prefill_of_a_flat_tail(cuda_device, t, queries, n, heads, split):
+    d = 64
+    q, k, v = tail(n, 1, d, t)
+    assert (moe.load_library().amoe_attn_prefill_workspace(d, 0, heads, 1, queries, n, 1) > 0) == split
+    qs = q.expand(queries, heads, d).contiguous()
+    got = attention.prefill(qs.cuda(), k.cuda(), v.cuda(), i32([0, queries]).cuda(), i32([0, n]).cuda(), scale=1.0)
+    want, bound = R.attention(qs[:, :1], k, v, scale=1.0)
+    for h in (0, heads - 1):
+        R.close(got[:, h:h + 1], want, bound + tail_bound(n))
