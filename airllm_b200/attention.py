@@ -5,7 +5,7 @@ The operators of the GPT-OSS layer's attention half between its two projections
 (internal/model/gptoss/layer.go:40-92, internal/backend/cpuref/attention.go:11-171,
 rope.go:10-86).  A serving loop holds one ``KVCache`` a layer, all over one page table:
 
-    rope = Rope(64, 150000.0)
+    rope = Rope.yarn(64, 150000.0)
     cache = KVCache(pages, 64, kv_heads=8, head_dim=64, dtype=torch.float8_e4m3fn)
     # a prompt: packed rows of all sequences, cu their starts
     q = cache.append(k, v, table, past, cu, q=q, rope=rope, k_out=kr)   # kr: the rotated keys
@@ -134,13 +134,34 @@ def _attn(scale, window: int, sinks, heads: int, device: int) -> bytes:
 
 
 class Rope:
-    """Rotary frequencies (RoPE, or GPT-OSS's YaRN: rope.go:10-44)."""
+    """Rotary frequencies, equal to the reference's: RoPE (yarn=False) or its YaRN table (rope.go:10-44).
+
+    The reference's YaRN table is not the published one: it divides the fast pairs by the factor instead of
+    the slow ones.  It is for results that have to equal the reference's; ``Rope.yarn`` makes the
+    frequencies that GPT-OSS and other models were trained with."""
 
     def __init__(self, head_dim: int, theta: float = 150000.0, yarn: bool = True):
-        lib = load_library()
+        lib = self._new()
+        _check(lib, lib.amoe_rope_init(head_dim, theta, 1 if yarn else 0, self._at))
+
+    @classmethod
+    def yarn(cls, head_dim: int, theta: float = 150000.0, factor: float = 32.0, original_context: float = 4096.0,
+             beta_fast: float = 32.0, beta_slow: float = 1.0, truncate: bool = False,
+             concentration: float | None = None) -> "Rope":
+        """YaRN as published (amoe_rope_init_yarn); the defaults are GPT-OSS's.  ``truncate`` rounds the
+        ramp's corners, as some models' configurations ask; concentration None: 1 + 0.1 ln(factor)."""
+        self = cls.__new__(cls)
+        lib = self._new()
+        _check(lib, lib.amoe_rope_init_yarn(head_dim, theta, factor, original_context, beta_fast, beta_slow,
+                                            1 if truncate else 0, self._at))
+        if concentration is not None:
+            self._c.concentration = concentration
+        return self
+
+    def _new(self):
         self._c = AmoeRope()
         self._at = ctypes.addressof(self._c)
-        _check(lib, lib.amoe_rope_init(head_dim, theta, 1 if yarn else 0, self._at))
+        return load_library()
 
     @property
     def frequencies(self) -> list:

@@ -312,6 +312,21 @@ cudaError_t launch_append_d(const AppendParams &p, int src, int cache, cudaStrea
     return launch_append<D, AMOE_GGUF_BF16>(p, cache, st);
 }
 
+int check_rope(int head_dim, double theta, const amoe_rope *out) {
+    if (!out) return reject("out must not be NULL");
+    if (head_dim <= 0 || head_dim % 2) return reject("rope head dimension must be positive and even");
+    if (head_dim > 2 * AMOE_ROPE_MAX_HALF)
+        return reject("rope head dimension above " + std::to_string(2 * AMOE_ROPE_MAX_HALF));
+    if (!(theta > 0) || std::isinf(theta)) return reject("rope theta must be finite and positive");
+    return AMOE_OK;
+}
+
+// The pair (not a whole one) that turns beta times within the original context.
+double yarn_corner(int head_dim, double theta, double original, double beta) {
+    const double pi = 3.14159265358979323846;
+    return head_dim * std::log(original / (beta * 2.0 * pi)) / (2.0 * std::log(theta));
+}
+
 template <int D>
 cudaError_t launch_read_d(const ReadParams &p, int cache, cudaStream_t st) {
     const int grid = (p.tokens - 1) / (kReadTokens * kReadThreads / 32) + 2;
@@ -331,24 +346,42 @@ using namespace amoe::attn;
 extern "C" {
 
 int amoe_rope_init(int32_t head_dim, double theta, int32_t yarn, amoe_rope *out) {
-    if (!out) return reject("out must not be NULL");
-    if (head_dim <= 0 || head_dim % 2) return reject("rope head dimension must be positive and even");
-    if (head_dim > 2 * AMOE_ROPE_MAX_HALF)
-        return reject("rope head dimension above " + std::to_string(2 * AMOE_ROPE_MAX_HALF));
-    if (!(theta > 0) || std::isinf(theta)) return reject("rope theta must be finite and positive");
+    if (int rc = check_rope(head_dim, theta, out)) return rc;
     *out = {};
     const int half = head_dim / 2;
-    const double factor = 32.0, original = 4096.0, pi = 3.14159265358979323846;
-    auto corner = [&](double beta) { return head_dim * std::log(original / (beta * 2.0 * pi)) / (2.0 * std::log(theta)); };
-    const double low = std::fmax(0.0, std::floor(corner(32.0)));
-    const double high = std::fmin(half - 1.0, std::ceil(corner(1.0)));
+    const double factor = 32.0, original = 4096.0;
+    const double low = std::fmax(0.0, std::floor(yarn_corner(head_dim, theta, original, 32.0)));
+    const double high = std::fmin(half - 1.0, std::ceil(yarn_corner(head_dim, theta, original, 1.0)));
     for (int i = 0; i < half; ++i) {
         out->freq[i] = std::pow(theta, -2.0 * i / head_dim);
         if (!yarn) continue;
         const double ramp = high == low ? 0.0 : std::fmax(0.0, std::fmin(1.0, (i - low) / (high - low)));
-        out->freq[i] *= ramp + (1.0 - ramp) / factor;
+        out->freq[i] *= ramp + (1.0 - ramp) / factor;  // the reference's ends, not the published ones
     }
     out->concentration = yarn ? 1.0 + 0.1 * std::log(factor) : 1.0;
+    out->head_dim = head_dim;
+    return AMOE_OK;
+}
+
+int amoe_rope_init_yarn(int32_t head_dim, double theta, double factor, double original_context, double beta_fast,
+                        double beta_slow, int32_t truncate, amoe_rope *out) {
+    if (int rc = check_rope(head_dim, theta, out)) return rc;
+    if (!(theta > 1)) return reject("yarn theta must be above 1");
+    if (!(factor >= 1) || std::isinf(factor)) return reject("yarn factor must be finite and at least 1");
+    if (!(original_context > 0) || std::isinf(original_context))
+        return reject("yarn original_context must be finite and positive");
+    if (!(beta_slow > 0) || !(beta_fast >= beta_slow) || std::isinf(beta_fast))
+        return reject("yarn beta_fast must be finite and at least beta_slow, beta_slow positive");
+    *out = {};
+    double low = yarn_corner(head_dim, theta, original_context, beta_fast);
+    double high = yarn_corner(head_dim, theta, original_context, beta_slow);
+    if (truncate) low = std::floor(low), high = std::ceil(high);
+    low = std::fmax(low, 0.0), high = std::fmin(high, head_dim - 1.0);
+    for (int i = 0; i < head_dim / 2; ++i) {
+        const double ramp = i <= low ? 0.0 : i >= high ? 1.0 : (i - low) / (high - low);
+        out->freq[i] = std::pow(theta, -2.0 * i / head_dim) * (1.0 - ramp + ramp / factor);
+    }
+    out->concentration = 1.0 + 0.1 * std::log(factor);
     out->head_dim = head_dim;
     return AMOE_OK;
 }

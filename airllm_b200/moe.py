@@ -122,6 +122,7 @@ SIGNATURES = {
     "amoe_head_next_token": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp]),
     "amoe_head_next_token_device": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp, _vp]),
     "amoe_rope_init": (ctypes.c_int, [_i32, ctypes.c_double, _i32, _vp]),
+    "amoe_rope_init_yarn": (ctypes.c_int, [_i32, *[ctypes.c_double] * 5, _i32, _vp]),
     "amoe_kv_append": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "amoe_kv_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "amoe_attn_prefill": (ctypes.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp,

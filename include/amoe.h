@@ -370,9 +370,21 @@ typedef struct amoe_rope {
     int32_t head_dim;
 } amoe_rope;
 
-/* Replaces: the frequency tables of RoPE and YaRNRoPE (rope.go:10-44; yarn != 0: GPT-OSS's
- * factor 32 over an original context of 4096).  No GPU needed.  head_dim even, 2..128. */
+/* Replaces: the frequency tables of RoPE and YaRNRoPE (rope.go:10-44; yarn != 0: factor 32 over
+ * an original context of 4096).  No GPU needed.  head_dim even, 2..128.
+ * The reference's YaRN table is not the published one, although it has GPT-OSS's numbers: it divides
+ * the fast pairs by the factor and leaves the slow ones, and rounds the ramp's corners.  It is for
+ * results that have to equal the reference's; weights trained with YaRN want amoe_rope_init_yarn. */
 AMOE_API int amoe_rope_init(int32_t head_dim, double theta, int32_t yarn, amoe_rope *out);
+
+/* No counterpart in the reference: YaRN as published (arXiv 2309.00071, "NTK-by-parts").  Pair i turns by
+ * theta^(-2i/head_dim) * (1 - r + r / factor) a token; r is 0 for pairs that turn beta_fast times or more
+ * within original_context, 1 for those that turn beta_slow times or less, and linear in i between
+ * the two corners (truncate != 0: the first rounded down, the second up).  The concentration is
+ * 1 + 0.1 ln(factor); a caller may overwrite it.  GPT-OSS: theta 150000, factor 32, original_context 4096,
+ * beta_fast 32, beta_slow 1, truncate 0.  theta > 1, factor >= 1, beta_fast >= beta_slow > 0. */
+AMOE_API int amoe_rope_init_yarn(int32_t head_dim, double theta, double factor, double original_context,
+                                 double beta_fast, double beta_slow, int32_t truncate, amoe_rope *out);
 
 /* Replaces: yarnHeads (layer.go:189-207) and KVCache.Append (attention.go:40-59).  Packed
  * new tokens: rows cu[s] .. cu[s+1] - 1 of q, k and v (cu [seqs + 1], device) belong to

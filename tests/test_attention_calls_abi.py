@@ -1,9 +1,10 @@
 """Calls of the attention entry points that the documentation allows, on the host side (no GPU)."""
 import ctypes
+import math
 
 import pytest
 
-from airllm_b200 import moe
+from airllm_b200 import AmoeError, attention, moe
 
 F16, BF16 = moe.GGUF_F16, moe.GGUF_BF16
 AT = 1 << 20  # an aligned address that no refused call reads
@@ -53,3 +54,71 @@ def test_append_of_more_tokens_than_a_grid_holds():
     assert lib.amoe_kv_append(ref(c), ref(s), AT, AT, 2 ** 31 - 1, None, None, ref(flat), ref(flat), None, None, None,
                               None) == moe.AMOE_ERR_INVALID
     assert "tokens" in last_error()
+
+
+def published_yarn(d, theta, factor, context, fast, slow, truncate):
+    """Frequencies by the paper's formula: a pair's turns within the original context decide."""
+    out = []
+    corner = [d / 2 * math.log(context / (2 * math.pi * beta), theta) for beta in (fast, slow)]
+    if truncate:
+        corner = [math.floor(corner[0]), math.ceil(corner[1])]
+    low, high = max(corner[0], 0), min(corner[1], d - 1)
+    for i in range(d // 2):
+        base = 1.0 / theta ** (i / (d / 2))
+        keep = 1 - min(max((i - low) / (high - low), 0.0), 1.0)  # how much of the pair is left as it is
+        out.append(keep * base + (1 - keep) * base / factor)
+    return out
+
+
+@pytest.mark.parametrize("d,theta,factor,context,fast,slow,truncate", [
+    (64, 150000.0, 32.0, 4096.0, 32.0, 1.0, 0), (128, 150000.0, 32.0, 4096.0, 32.0, 1.0, 0),
+    (128, 1e6, 4.0, 32768.0, 32.0, 1.0, 1), (64, 10000.0, 40.0, 4096.0, 32.0, 1.0, 1), (2, 10000.0, 8.0, 4096.0, 32.0, 1.0, 0),
+    (96, 500000.0, 1.0, 8192.0, 16.0, 2.0, 0)])
+def test_yarn_frequencies_are_the_published_ones(d, theta, factor, context, fast, slow, truncate):
+    rope = moe.AmoeRope()
+    assert moe.load_library().amoe_rope_init_yarn(d, theta, factor, context, fast, slow, truncate, ref(rope)) == moe.AMOE_OK
+    got, want = list(rope.freq)[:d // 2], published_yarn(d, theta, factor, context, fast, slow, truncate)
+    # a handful of float64 roundings on either side
+    for a, b in zip(got, want):
+        assert abs(a - b) <= 2.0 ** -48 * b
+    assert got[0] == 1.0  # the fastest pair is left as it is
+    if d >= 64:  # and the slowest divided
+        assert abs(got[-1] - theta ** (2 / d - 1) / factor) <= 2.0 ** -48 * got[-1]
+    assert abs(rope.concentration - (1 + 0.1 * math.log(factor))) <= 2.0 ** -50 and rope.head_dim == d
+
+
+def test_yarn_with_every_pair_fast_or_slow():
+    lib, rope = moe.load_library(), moe.AmoeRope()
+    # a context so long that every pair turns often enough, and one in which none turns once
+    assert lib.amoe_rope_init_yarn(64, 1e4, 8.0, 1e12, 32.0, 1.0, 0, ref(rope)) == moe.AMOE_OK
+    assert all(abs(f * 1e4 ** (i / 32) - 1) < 1e-12 for i, f in enumerate(list(rope.freq)[:32]))
+    assert lib.amoe_rope_init_yarn(64, 1e4, 8.0, 3.0, 32.0, 1.0, 0, ref(rope)) == moe.AMOE_OK
+    assert all(abs(f * 8 * 1e4 ** (i / 32) - 1) < 1e-12 for i, f in enumerate(list(rope.freq)[:32]) if i > 0)
+
+
+def test_the_reference_table_is_kept_under_its_own_name():
+    """YaRNRoPE's ends of the ramp (rope.go:17-44) are the other way round."""
+    rope = moe.AmoeRope()
+    assert moe.load_library().amoe_rope_init(64, 150000.0, 1, ref(rope)) == moe.AMOE_OK
+    assert rope.freq[0] == 1 / 32 and abs(rope.freq[31] * 150000.0 ** (31 / 32) - 1) < 1e-12
+
+
+@pytest.mark.parametrize("at,value,word", [
+    (0, 63, "even"), (0, 256, "128"), (1, 1.0, "theta"), (1, math.inf, "theta"), (2, 0.5, "factor"), (2, math.nan, "factor"),
+    (2, math.inf, "factor"), (3, 0.0, "original_context"), (3, math.inf, "original_context"), (4, 0.5, "beta_fast"),
+    (4, math.inf, "beta_fast"), (5, 0.0, "beta_slow"), (5, math.nan, "beta_slow")])
+def test_yarn_refusals(at, value, word):
+    args = [64, 150000.0, 32.0, 4096.0, 32.0, 1.0, 0]
+    args[at] = value
+    assert moe.load_library().amoe_rope_init_yarn(*args, ref(moe.AmoeRope())) == moe.AMOE_ERR_INVALID
+    assert word in last_error()
+
+
+def test_rope_from_python():
+    rope = attention.Rope.yarn(64, 150000.0)
+    assert rope.frequencies[0] == 1.0 and len(rope.frequencies) == 32
+    assert abs(rope.concentration - 1.3465735902799727) < 1e-12
+    assert attention.Rope.yarn(128, 1e6, factor=4.0, original_context=32768, truncate=True, concentration=1.0).concentration == 1.0
+    with pytest.raises(AmoeError, match="factor"):
+        attention.Rope.yarn(64, factor=0.0)
+    assert attention.Rope(64, 150000.0).frequencies[0] == 1 / 32  # the reference's table

@@ -136,3 +136,34 @@ def test_prefill_of_a_flat_tail(cuda_device, t, queries, n, heads, split):
     want, bound = R.attention(qs[:, :1], k, v, scale=1.0)
     for h in (0, heads - 1):
         R.close(got[:, h:h + 1], want, bound + tail_bound(n))
+
+
+# ---- rotation ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("d,yarn", [(64, True), (128, True), (64, False), (128, False)])
+def test_append_rotates_by_the_published_frequencies(cuda_device, d, yarn):
+    """Frequencies computed here, not taken from the object under test."""
+    g = gen(71)
+    theta = 150000.0
+    freq, conc = [1.0 / theta ** (2 * i / d) for i in range(d // 2)], 1.0
+    if yarn:
+        low, high = (d / 2 * math.log(4096 / (2 * math.pi * beta)) / math.log(theta) for beta in (32, 1))
+        freq = [f * (1 - r + r / 32) for f, r in zip(freq, (min(max((i - low) / (high - low), 0), 1) for i in range(d // 2)))]
+        conc = 1 + 0.1 * math.log(32)
+        assert freq[0] == 1.0 and abs(freq[-1] * 32 * theta ** (1 - 2 / d) - 1) < 1e-12
+    rope = attention.Rope.yarn(d, theta) if yarn else attention.Rope(d, theta, yarn=False)
+    new, past, page = [3, 70, 1], [131000, 0, 4096], 128
+    table, pool = table_for(g, [a + b for a, b in zip(new, past)], page)
+    n = sum(new)
+    x = randn(g, n, 6, d)
+    cache = attention.KVCache(pool, page, 1, d, dtype=BF16)
+    k_out = torch.empty(n, 1, d, device="cuda")
+    q = cache.append(x[:, 4:5].cuda(), x[:, 5:].cuda(), table.cuda(), i32(past).cuda(), starts(new).cuda(), q=x[:, :4].cuda(),
+                     rope=rope, k_out=k_out)
+    cache.check()
+    pos = torch.cat([torch.arange(p, p + m) for m, p in zip(new, past)])
+    # A frequency is within 2^-48 of the one computed here, an angle within pos 2^-48, and an element turns by that times
+    # its pair's length; both sides round to float32 once.
+    far = x[:, :5].double().abs().amax() * math.sqrt(2) * conc * pos.max() * 2.0 ** -48
+    want = R.rotated(x[:, :5], pos, freq, conc).double()
+    got = torch.cat((q, k_out), 1).cpu().double()
+    assert ((got - want).abs() <= 2.0 ** -23 * want.abs() + far).all()
