@@ -46,35 +46,44 @@ struct CacheDev {
     int table_stride, shift, heads;  // page_size = 1 << shift
 };
 
-// The sequence of packed row t: the last s with cu[s] <= t (empty sequences before it
-// share its start).  Always in [0, seqs), whatever cu holds.
-__host__ __device__ inline int find_seq(const int32_t *cu, int seqs, int t) {
-    int lo = 0, hi = seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (cu[mid] <= t) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
-// The same for N rows t, t + 1, ... by a whole warp, a load for every 32 sequences instead of a chain of them.
-// Starts that decrease give some sequence in [0, seqs) here too; the caller checks that it holds the row.
+// The sequences of packed rows t, t + 1, ... t + N - 1: how many end at or before each (empty sequences before a row's
+// share its start).  Always in [0, seqs), whatever cu holds; the caller checks that the sequence holds the row.  A whole
+// warp calls it, with a load for every 32 sequences instead of a chain of them; the host, for checks, looks at the same
+// 32 in turn.
 template <int N>
-__device__ __forceinline__ void find_seqs(const int32_t *cu, int seqs, int t, int (&s)[N]) {
-    const int lane = threadIdx.x % 32;
+__host__ __device__ __forceinline__ void find_seqs(const int32_t *cu, int seqs, int t, int (&s)[N]) {
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k] = 0;
     for (int s0 = 0; s0 < seqs; s0 += 32) {
-        const int end = s0 + lane < seqs ? cu[s0 + lane + 1] : INT_MAX;
-        uint32_t behind = 0;
+        auto end_of = [&](int i) { return s0 + i < seqs ? cu[s0 + i + 1] : INT_MAX; };
+#ifdef __CUDA_ARCH__
+        const int end = end_of(threadIdx.x % 32);
+        auto ended = [&](int row) { return __ballot_sync(0xffffffffu, end <= row); };
+        auto count = [](uint32_t bits) { return __popc(bits); };
+#else
+        auto ended = [&](int row) {
+            uint32_t bits = 0;
+            for (int i = 0; i < 32; ++i) bits |= (uint32_t)(end_of(i) <= row) << i;
+            return bits;
+        };
+        auto count = [](uint32_t bits) { return __builtin_popcount(bits); };
+#endif
+        uint32_t bits = 0;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            behind = __ballot_sync(0xffffffffu, end <= t + k);
-            s[k] = min(s[k] + __popc(behind), seqs - 1);
+            bits = ended(t + k);
+            const int upto = s[k] + count(bits);
+            s[k] = upto < seqs ? upto : seqs - 1;
         }
-        if (behind != 0xffffffffu) break;  // the last row's sequence, and so every one's, is found
+        if (bits != 0xffffffffu) break;  // the last row's sequence, and so every one's, is found
     }
+}
+
+// One row's, on the host.
+inline int find_seq(const int32_t *cu, int seqs, int t) {
+    int s[1];
+    find_seqs(cu, seqs, t, s);
+    return s[0];
 }
 
 // Page of position pos (>= 0) of sequence s, or the negated status bit where the table has none.

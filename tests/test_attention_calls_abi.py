@@ -1,11 +1,14 @@
 """Calls of the attention entry points that the documentation allows, on the host side (no GPU)."""
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 
-from airllm_b200 import AmoeError, attention, moe
+from airllm_b200 import AmoeError, attention, build, moe
 
+CUDA = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cuda")
 F16, BF16 = moe.GGUF_F16, moe.GGUF_BF16
 AT = 1 << 20  # an aligned address that no refused call reads
 
@@ -122,3 +125,11 @@ def test_rope_from_python():
     with pytest.raises(AmoeError, match="factor"):
         attention.Rope.yarn(64, factor=0.0)
     assert attention.Rope(64, 150000.0).frequencies[0] == 1 / 32  # the reference's table
+
+
+def test_the_search_for_sequences(tmp_path):
+    exe = str(tmp_path / "kv_search")
+    subprocess.run([build.NVCC, *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr", "-I", build.INCLUDE, "-I", build.CSRC,
+                    "-o", exe, os.path.join(CUDA, "kv_search_check.cu")], check=True)
+    got = subprocess.run([exe], capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout.strip() == "ok", got.stdout
