@@ -26,12 +26,14 @@
 // split over CTAs, and a second kernel joins the partial sums (`layout` below chooses, with what it measured).
 //
 // The maximum is lazy: O and the sum are rescaled only when a row's maximum has grown by more
-// than 2^8 since the last time, which float32 sums hold without loss.  Weights are 2^(score - maximum) in bf16, and 2^7
-// times that in f16 (attn.cuh: weight_shift).
+// than 2^8 (2^4 in f16, whose weights carry a factor: attn.cuh) since the last time, which float32 sums hold without loss.
 //
-// A key that a row must not see has weight 0, but 0 times an infinity or NaN in its value is NaN.
-// Values behind the tile's last visible key are overwritten with zeros in shared memory; a row whose
-// result is still not finite is computed again by its thread, key by visible key.  Finite inputs never take that path.
+// A key that a row must not see has weight 0, but 0 times an infinity or NaN in its value is NaN.  Values behind the
+// tile's last visible key are overwritten with zeros in shared memory.  Where a row's result still is not finite the CTA
+// does its tiles once more, and the feeding warp now takes out what is not finite among the keys that only some of the
+// rows see (at the diagonal and at the window's edge); the rows that see such a key add its value at the end, for with any weight
+// above zero the sum is that infinity or NaN.  Finite inputs never go that way, others take about twice the time at most
+// (4096 tokens 220 us, with one infinity 273, all NaN 486; looking through those keys at once cost windows 8 to 35 %).
 #include "attn.cuh"
 #include "tc_ptx.cuh"
 
@@ -50,10 +52,11 @@ using bs::tc_fence_after;
 using bs::tc_fence_before;
 
 constexpr int kRows = 128;
+constexpr int kStages = 2, kBars = 5 + 2 * kStages;
 constexpr int kSoftWarps = 4, kFeedWarp = 4, kThreads = 160;
 
 struct PrefillParams {
-    RowsDev q, k, v, out;  // K and V for the rows that are computed again
+    RowsDev v, out;
     const int32_t *cu_q, *cu_k;
     const float *sinks;
     float scale_log2;
@@ -67,7 +70,6 @@ template <int D>
 struct Cfg {
     static constexpr int N = 64;                  // keys of a tile
     static constexpr int kHalves = D / 64;        // 128-byte column blocks of a row
-    static constexpr int kStages = 2;
     static constexpr int kQBytes = kRows * D * 2;
     static constexpr int kTileBytes = N * D * 2;
     static constexpr int kCtas = D == 64 ? 3 : 2;  // to an SM
@@ -87,6 +89,7 @@ struct Work {
     int tok0, tokens;    // first query row and how many of the tile's are the sequence's
     int at0;             // position of the first among its keys
     int k0, lo, hi;      // the sequence's first key row; the tile's visible keys [lo, hi), or this CTA's part of them
+    int odd;             // values that are not finite were left out of the careful pass's products
     int dead;            // a bounded wait gave up
     int found;
 };
@@ -192,6 +195,13 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The larger, NaN where one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // Two float32 lanes in one instruction.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -216,10 +226,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 
 // 2^x of two values on the FMA pipe, to 2^-23: with n the integer next to x (read from the low bits of
 // x + 1.5 * 2^23) and f = x - n in [-1/2, 1/2], 2^f by a polynomial of degree 5 fitted to the least relative error,
-// and n added to its exponent.  Below -127 the result is a zero or the smallest subnormal; NaN gives no finite 16-bit value.
+// and n added to its exponent.  Below -127 the result is a zero or the smallest subnormal, and so is it for NaN.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+    x.x = fmaxf(x.x, -127.0f), x.y = fmaxf(x.y, -127.0f);
     const uint64_t v = pair(x.x, x.y), big = pair(12582912.0f, 12582912.0f);
     const uint64_t t = add2(v, big);
     const uint64_t f = fma2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), v);
@@ -270,7 +279,7 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, int par
                 w->hi = min(w->hi, w->lo + t1 * N);
                 w->lo = min(w->lo + t0 * N, w->hi);
             }
-            w->dead = 0;
+            w->odd = w->dead = 0;
         }
         if (__any_sync(0xffffffffu, mine)) return true;
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -284,115 +293,95 @@ __device__ __forceinline__ float sink_weight(float sink, float z) {
     return sink == INFINITY ? NAN : ex2(sink * kLog2e - z);
 }
 
-// A row again, key by visible key: for results that are not finite.  Its arrays stay in local memory (no loop is
-// unrolled), so that the path costs the kernel no registers.
-template <int D, int TYPE>
-__device__ __forceinline__ void row_again(const PrefillParams &p, int tok, int head, int k0, int from, int at) {
-    float acc[D], m = -INFINITY, l = 0.0f;
-    const int kvh = head / p.group;
-    const char *q = p.q.p + tok * p.q.ts + head * p.q.hs;
-    float x[8], y[8];
+// Zeros in the place of a word's elements that are not finite; true where there was one.
+template <int TYPE>
+__device__ __forceinline__ bool drop_odd(uint32_t &w) {
+    constexpr uint32_t EXP = TYPE == AMOE_GGUF_F16 ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t ONE = TYPE == AMOE_GGUF_F16 ? 0x04000400u : 0x00800080u;  // carries a full exponent into the sign's place
+    const uint32_t odd = ((w & EXP) + ONE) >> 15 & 0x00010001u;
+    w &= ~(odd * 0xffffu);
+    return odd != 0;
+}
+
+// The keys that all of a tile's rows see: [from, to).
+struct Shared {
+    int from, to;
+};
+__device__ __forceinline__ Shared shared_keys(int window, int at0, int tokens) {
+    return {window > 0 ? at0 + tokens - window : 0, at0 + 1};
+}
+
+// What drop_odd took out of 32 elements of a row that sees the keys [from, to).  v: the row and elements of key 0.
+template <int TYPE>
+__device__ __forceinline__ void add_odd(float (&o)[32], const char *v, int64_t step, int from, int to, Shared all) {
 #pragma unroll 1
-    for (int d = 0; d < D; ++d) acc[d] = 0.0f;
-#pragma unroll 1
-    for (int j = from; j <= at; ++j) {
-        const char *k = p.k.p + (k0 + j) * p.k.ts + kvh * p.k.hs, *v = p.v.p + (k0 + j) * p.v.ts + kvh * p.v.hs;
-        float dot = 0.0f;
-#pragma unroll 1
-        for (int d = 0; d < D; d += 8) {
-            load8<TYPE>(q + d * 2, x);
-            load8<TYPE>(k + d * 2, y);
-            for (int i = 0; i < 8; ++i) dot = fmaf(x[i], y[i], dot);
+    for (int j = from; j < to; ++j) {
+        if (j >= all.from && j < all.to) {
+            j = all.to - 1;
+            continue;
         }
-        const float s = dot * p.scale_log2, mm = fmaxf(m, s), z = mm == -INFINITY ? 0.0f : mm;
-        const float keep = exp2f(m - z), e = exp2f(s - z);
-        m = mm;
-        l = l * keep + e;
-#pragma unroll 1
-        for (int d = 0; d < D; d += 8) {
-            load8<TYPE>(v + d * 2, x);
-            for (int i = 0; i < 8; ++i) acc[d + i] = acc[d + i] * keep + e * x[i];
+        const char *row = v + j * step;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            float x[8];
+            load8<TYPE>(row + i * 2, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[i + e] += isfinite(x[e]) ? 0.0f : x[e];
         }
-    }
-    const float z = m == -INFINITY ? 0.0f : m;
-    if (p.sinks) l += sink_weight(p.sinks[head], z);
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll 1
-    for (int d = 0; d < D; d += 8) {
-        for (int i = 0; i < 8; ++i) x[i] = acc[d + i] * by;
-        store8<TYPE>(p.out.p + tok * p.out.ts + head * p.out.hs + d * 2, x);
     }
 }
 
-// SPLIT: the keys of tiles from p.whole on are split over p.split CTAs (windowed calls of many tiles, which a CTA's start bounds, took 4 %
-// longer where one kernel did both).
-template <int D, int TYPE, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
-    prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
-    using C = Cfg<D>;
-    constexpr int N = C::N, HALVES = C::kHalves, kStages = C::kStages;
+// Where a CTA's shared memory lies and which tile it has, of which part of the keys (-1: all).
+struct Cta {
+    uint8_t *sm;
+    uint64_t *bars;
+    uint32_t *tmem_slot;
+    uint32_t tmem, tmem_p;  // S and O; P
+    Work *work;
+    int tile, part;
+};
+// The columns' addresses, once they are allocated.
+template <int D>
+__device__ __forceinline__ void find_tmem(Cta &c) {
+    c.tmem = c.tmem_slot[0], c.tmem_p = Cfg<D>::kTmemP ? c.tmem_slot[1] : c.tmem + Cfg<D>::kP;
+}
+template <int D, bool SPLIT>
+__device__ __forceinline__ Cta this_cta(const PrefillParams &p) {
     extern __shared__ __align__(1024) uint8_t sm_raw[];
-    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *q_s = sm, *k_s = q_s + C::kQBytes, *v_s = k_s + kStages * C::kTileBytes;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(v_s + kStages * C::kTileBytes);
-    uint64_t *q_full = bars, *k_full = bars + 1, *v_full = k_full + kStages, *s_full = v_full + kStages;
-    uint64_t *s_free = s_full + 1, *p_full = s_free + 1, *o_done = p_full + 1;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_done + 1);
-    Work *work = reinterpret_cast<Work *>(tmem_slot + 2);
+    Cta c;
+    c.sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
+    c.bars = reinterpret_cast<uint64_t *>(c.sm + Cfg<D>::kQBytes + 2 * kStages * Cfg<D>::kTileBytes);
+    c.tmem_slot = reinterpret_cast<uint32_t *>(c.bars + kBars);
+    c.work = reinterpret_cast<Work *>(c.tmem_slot + 2);
+    c.tile = blockIdx.x, c.part = -1;
+    if (SPLIT && c.tile >= p.whole) {
+        c.part = (c.tile - p.whole) % p.split;
+        c.tile = p.whole + (c.tile - p.whole) / p.split;
+    }
+    return c;
+}
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    int tile = blockIdx.x, part = -1;
-    if (SPLIT && tile >= p.whole) {
-        part = (tile - p.whole) % p.split;
-        tile = p.whole + (tile - p.whole) / p.split;
-    }
-    const int kvh = tile % p.kv_heads;
-    // the work is found while the TMEM columns, the barriers and the tensor maps are made ready
-    if (warp == 0) {
-        const bool f = find_work<N>(p, tile / p.kv_heads, part, work);
-        if (lane == 0) work->found = f;
-    } else if (warp == 1) {
-        if (lane == 0) {
-            mbar_init(q_full, 1);
-            for (int i = 0; i < kStages; ++i) mbar_init(k_full + i, 1), mbar_init(v_full + i, 1);
-            mbar_init(s_full, 1), mbar_init(o_done, 1);
-            mbar_init(s_free, kSoftWarps), mbar_init(p_full, kSoftWarps);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-    } else if (warp == kFeedWarp) {
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_q) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
-        }
-        __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "n"(C::kTmemCols)
-                     : "memory");
-        if (C::kTmemP)
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot + 1)),
-                         "n"(C::kTmemP ? C::kTmemP : 32)
-                         : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot, tmem_p = C::kTmemP ? tmem_slot[1] : tmem + C::kP;
-    auto leave = [&]() {
-        if (warp != kFeedWarp) return;
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kTmemCols));
-        if (C::kTmemP)
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_p),
-                         "n"(C::kTmemP ? C::kTmemP : 32));
-    };
-    if (SPLIT) cudaTriggerProgrammaticLaunchCompletion();  // lets the join take the places that fall free
-    if (!work->found) {
-        leave();
-        return;
-    }
+// Barriers: q_full, k_full[2], v_full[2], s_full, s_free, p_full, o_done.
+__device__ __forceinline__ void init_bars(uint64_t *bars) {
+    for (int i = 0; i < kBars; ++i) mbar_init(bars + i, i == kBars - 3 || i == kBars - 2 ? kSoftWarps : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+
+// The CTA's tiles from the first to the last.  SPLIT: those from p.whole on have their keys split over p.split CTAs.  CAREFUL: once
+// more, with values that are not finite kept from rows that do not see them.  True where this thread's row has a sum
+// that is not finite.
+template <int D, int TYPE, bool SPLIT, bool CAREFUL>
+__device__ __forceinline__ bool tile_pass(const PrefillParams &p, const CUtensorMap *tm_q, const CUtensorMap *tm_k,
+                                          const CUtensorMap *tm_v, const Cta &cta) {
+    using C = Cfg<D>;
+    constexpr int N = C::N, HALVES = C::kHalves;
+    uint8_t *q_s = cta.sm, *k_s = q_s + C::kQBytes, *v_s = k_s + kStages * C::kTileBytes;
+    uint64_t *q_full = cta.bars, *k_full = q_full + 1, *v_full = k_full + kStages, *s_full = v_full + kStages;
+    uint64_t *s_free = s_full + 1, *p_full = s_free + 1, *o_done = p_full + 1;
+    Work *work = cta.work;
+    const uint32_t tmem = cta.tmem, tmem_p = cta.tmem_p;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tile = cta.tile, part = cta.part, kvh = tile % p.kv_heads;
+    bool odd_row = false;
     const int tok0 = work->tok0, at0 = work->at0, lo = work->lo, hi = work->hi, k0 = work->k0;
     const int tiles = hi > lo ? (hi - lo - 1) / N + 1 : 0;
     // columns of the last tile that hold a visible key, in whole MMA steps
@@ -409,17 +398,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                 tma_3d(ring + s * C::kTileBytes + h * N * 128, tm, full + s, h * 64, kvh, k0 + lo + j * N);
         };
         if (lane == 0 && tiles > 0) {
-            mbar_expect_tx(q_full, p.tile_tokens * p.group * D * 2);
-            for (int h = 0; h < HALVES; ++h) tma_3d(q_s + h * kRows * 128, &tm_q, q_full, h * 64, kvh * p.group, tok0);
+            if (!CAREFUL) {
+                mbar_expect_tx(q_full, p.tile_tokens * p.group * D * 2);
+                for (int h = 0; h < HALVES; ++h) tma_3d(q_s + h * kRows * 128, tm_q, q_full, h * 64, kvh * p.group, tok0);
+            }
             for (int j = 0; j < kStages && j < tiles; ++j) {
-                load(k_s, &tm_k, k_full, j);
-                load(v_s, &tm_v, v_full, j);
+                load(k_s, tm_k, k_full, j);
+                load(v_s, tm_v, v_full, j);
             }
         }
         __syncwarp();
         const uint64_t q_d = desc_sw128(smem_u32(q_s), 16), k_d = desc_sw128(smem_u32(k_s), 16);
         const uint64_t v_d = desc_sw128(smem_u32(v_s), N * 128);
-        bool ok = tiles > 0 && wait_warp(q_full, 0, work);
+        bool ok = tiles > 0 && (CAREFUL || wait_warp(q_full, 0, work));
         auto scores = [&](int j) {  // S = Q K^T of tile j
             if (j >= tiles) return;
             const int s = j % kStages;
@@ -434,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                 for (int i = 0; i < D / 16; ++i)
                     mma_ss(tmem + C::kS, q_d + i / 4 * (kRows * 8) + i % 4 * 2, kd + i / 4 * (N * 8) + i % 4 * 2, id, i > 0);
                 mma_commit(s_full);
-                if (j > 0 && j - 1 + kStages < tiles) load(k_s, &tm_k, k_full, j - 1 + kStages);
+                if (j > 0 && j - 1 + kStages < tiles) load(k_s, tm_k, k_full, j - 1 + kStages);
             }
             __syncwarp();
         };
@@ -445,12 +436,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
             if (!ok) return;
             const int cols = t + 1 == tiles ? last_cols : N;
             const int seen = hi - lo - t * N;
+            bool odd = false;
+            if (CAREFUL) {  // keys [0, edge) and [diag, end) of the tile are not for all rows
+                const int key = lo + t * N, end = min(seen, N);
+                const Shared all = shared_keys(p.window, at0, work->tokens);
+                const int edge = min(max(all.from - key, 0), end), diag = min(max(all.to - key, edge), end);
+                for (int i = lane; i < (edge + end - diag) * 8 * HALVES; i += 32) {
+                    const int r = i / (8 * HALVES), h = i / 8 % HALVES;
+                    uint4 *at = reinterpret_cast<uint4 *>(v_s + s * C::kTileBytes + h * N * 128 +
+                                                          (r < edge ? r : diag + r - edge) * 128 + i % 8 * 16);
+                    uint4 w = *at;
+                    bool here = drop_odd<TYPE>(w.x);
+                    here |= drop_odd<TYPE>(w.y);
+                    here |= drop_odd<TYPE>(w.z);
+                    here |= drop_odd<TYPE>(w.w);
+                    if (here) *at = w;
+                    odd |= here;
+                }
+                odd = __any_sync(0xffffffffu, odd);
+                if (odd) work->odd = 1;
+            }
             if (seen < cols) {  // no value behind the last visible key reaches the products
                 for (int i = lane; i < (cols - seen) * 8 * HALVES; i += 32) {
                     const int h = i / ((cols - seen) * 8), r = i / 8 % (cols - seen);
                     *reinterpret_cast<uint4 *>(v_s + s * C::kTileBytes + h * N * 128 + (seen + r) * 128 + i % 8 * 16) =
                         make_uint4(0, 0, 0, 0);
                 }
+            }
+            if (odd || seen < cols) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
@@ -464,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                 for (int i = 0; i < N / 16; ++i)
                     if (i * 16 < cols) mma_ts(tmem + C::kO, tmem_p + i * 8, vd + i * 128, id, t > 0 || i > 0);
                 mma_commit(o_done);
-                if (t > 0 && t - 1 + kStages < tiles) load(v_s, &tm_v, v_full, t - 1 + kStages);
+                if (t > 0 && t - 1 + kStages < tiles) load(v_s, tm_v, v_full, t - 1 + kStages);
             }
             __syncwarp();
         };
@@ -472,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
             scores(j);
             weigh(j - 1);
         }
+        if (CAREFUL) asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");  // work->odd is as it stays
     } else {
         // a thread's row: token r / group of the tile, query head r % group of the kv head
         const int r = threadIdx.x, tok = r / p.group, head = kvh * p.group + r % p.group, at = at0 + tok;
@@ -503,8 +517,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
             }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // chains short enough to overlap
 #pragma unroll
-            for (int i = 0; i < N; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            for (int i = 0; i < N; ++i) tops[i % 4] = max_nan(tops[i % 4], s[i]);
+            const float top = max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3]));
+            l = top < INFINITY ? l : NAN;  // a score of NaN or +inf, which not every form of 2^x passes on
             bool waited = j == 0;  // P and O are free once the products of the tile before are done
             if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > weight_lazy(TYPE))) {
                 const float mm = fmaxf(m, top);
@@ -556,40 +571,48 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
         }
         if (tiles > 0) ok &= wait_warp(o_done, (uint32_t)(tiles - 1) & 1u, work);
         tc_fence_after();
+        if (CAREFUL) asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
         const bool mine = tok < work->tokens && r < p.tile_tokens * p.group;
+        float worst = 0.0f;  // 0, or NaN
+        // 32 elements of the row's sums
+        auto row_of = [&](int c, float (&o)[32]) {
+            __syncwarp();
+            if (tiles > 0) {
+                bs::tmem_ld32(tmem + lanes + C::kO + c, o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+            }
+            if (CAREFUL && mine && work->odd)
+                add_odd<TYPE>(o, p.v.p + k0 * p.v.ts + kvh * p.v.hs + c * 2, p.v.ts,
+                              p.window > 0 ? max(lo, at - p.window + 1) : lo, min(at + 1, hi),
+                              shared_keys(p.window, at0, work->tokens));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;
+        };
         if (SPLIT && part >= 0) {  // the row's sums over this part, for the kernel that joins them
             float *sums = p.work + (int64_t)((tile - p.whole) * p.split + part) * (D + 2) * kRows + r;
             if (mine) {
                 sums[D * kRows] = m == -INFINITY ? -INFINITY : m * p.scale_log2 - SHIFT;
-                sums[(D + 1) * kRows] = ok ? l : NAN;
+                sums[(D + 1) * kRows] = l;
             }
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 float o[32];
-                __syncwarp();
-                if (tiles > 0) bs::tmem_ld32(tmem + lanes + C::kO + c, o);
+                row_of(c, o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (mine) sums[(c + i) * kRows] = tiles > 0 ? o[i] : 0.0f;
+                    if (mine) sums[(c + i) * kRows] = ok ? o[i] : NAN;
             }
         } else {
+            const bool none = m == -INFINITY && !isnan(l);  // the row saw nothing
             if (p.sinks && mine) l += sink_weight(p.sinks[head], m == -INFINITY ? 0.0f : m * p.scale_log2 - SHIFT);
-            // a row that saw nothing has no maximum (and may have a subnormal sum: ex2_poly's smallest)
-            const float by = !ok ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
+            const float by = !ok ? NAN : none ? 0.0f : 1.0f / l;
             char *dst = p.out.p + (int64_t)(tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs;
-            float worst = isnan(l) ? l : 0.0f;  // 0, or NaN
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 float o[32];
-                __syncwarp();
-                if (tiles > 0) {
-                    bs::tmem_ld32(tmem + lanes + C::kO + c, o);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) worst += o[i] * 0.0f;
+                row_of(c, o);
                 if (mine) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
@@ -600,28 +623,102 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
                     }
                 }
             }
-            if (mine && ok && worst != 0.0f)
-                row_again<D, TYPE>(p, tok0 + tok, head, k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
         }
+        odd_row = mine && worst != 0.0f;
+    }
+    return odd_row;
+}
+
+// Out of the kernel's line, so that it costs it no registers; what it can find again it is not given, which would go
+// through local memory.
+template <int D, int TYPE, bool SPLIT>
+__device__ __noinline__ void careful_pass(const PrefillParams &p, const CUtensorMap *tm_q, const CUtensorMap *tm_k,
+                                          const CUtensorMap *tm_v) {
+    tc_fence_after();
+    Cta cta = this_cta<D, SPLIT>(p);
+    find_tmem<D>(cta);
+    tile_pass<D, TYPE, SPLIT, true>(p, tm_q, tm_k, tm_v, cta);
+}
+
+// SPLIT: the keys of tiles from p.whole on are split over p.split CTAs (windowed calls of many tiles, which a CTA's start bounds, took 4 %
+// longer where one kernel did both).
+template <int D, int TYPE, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, Cfg<D>::kCtas)
+    prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PrefillParams p) {
+    using C = Cfg<D>;
+    Cta cta = this_cta<D, SPLIT>(p);
+    Work *work = cta.work;
+    uint32_t *tmem_slot = cta.tmem_slot;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // the work is found while the TMEM columns, the barriers and the tensor maps are made ready
+    if (warp == 0) {
+        const bool f = find_work<C::N>(p, cta.tile / p.kv_heads, cta.part, work);
+        if (lane == 0) work->found = f;
+    } else if (warp == 1) {
+        if (lane == 0) init_bars(cta.bars);
+    } else if (warp == kFeedWarp) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_q) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "n"(C::kTmemCols)
+                     : "memory");
+        if (C::kTmemP)
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot + 1)),
+                         "n"(C::kTmemP ? C::kTmemP : 32)
+                         : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    find_tmem<D>(cta);
+    auto leave = [&]() {
+        if (warp != kFeedWarp) return;
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(cta.tmem), "n"(C::kTmemCols));
+        if (C::kTmemP)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(cta.tmem_p),
+                         "n"(C::kTmemP ? C::kTmemP : 32));
+    };
+    if (SPLIT) cudaTriggerProgrammaticLaunchCompletion();  // lets the join take the places that fall free
+    if (!work->found) {
+        leave();
+        return;
+    }
+    bool odd = tile_pass<D, TYPE, SPLIT, false>(p, &tm_q, &tm_k, &tm_v, cta);
+    tc_fence_before();
+    odd = __syncthreads_or(odd);
+    if (odd && !work->dead) {
+        if (threadIdx.x == 0) {  // every phase of the barriers is over, and they begin anew
+            for (int i = 0; i < kBars; ++i)
+                asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(cta.bars + i)) : "memory");
+            init_bars(cta.bars);
+        }
+        __syncthreads();
+        careful_pass<D, TYPE, SPLIT>(p, &tm_q, &tm_k, &tm_v);
+        tc_fence_before();
+        __syncthreads();
+    }
     leave();
 }
 
 // The join of the parts' sums.  A CTA takes 32 rows of a tile, a lane a row, a warp eight of the row's elements: sums are
-// read along the rows, as they were written, and a thread's loads do not wait for one another.
-constexpr int kJoinBlocks = kRows / 32;
+// read along the rows, as they were written, and a thread's loads do not wait for one another: two CTAs an SM are asked for
+// so that the compiler takes registers for them (16 queries behind 32768 keys 41 us with 40 registers, 34 with 63).
+constexpr int kJoinBlocks = kRows / 32, kJoinParts = 4;
 template <int D, int TYPE>
-__global__ void __launch_bounds__(D * 4) prefill_join_kernel(const __grid_constant__ PrefillParams p) {
+__global__ void __launch_bounds__(D * 4, 2) prefill_join_kernel(const __grid_constant__ PrefillParams p) {
     __shared__ Work work;
-    __shared__ int again[32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int tile = p.whole + blockIdx.x / kJoinBlocks, kvh = tile % p.kv_heads;
     if (warp == 0) {
         const bool f = find_work<Cfg<D>::N>(p, tile / p.kv_heads, -1, &work);
         if (lane == 0) work.found = f;
-        again[lane] = 0;
     }
     __syncthreads();
     // Launched while the partial sums are still being made.  CTAs without work wait as well: what follows on the stream waits
@@ -629,34 +726,41 @@ __global__ void __launch_bounds__(D * 4) prefill_join_kernel(const __grid_consta
     cudaGridDependencySynchronize();
     if (!work.found) return;
     const int r = blockIdx.x % kJoinBlocks * 32 + lane, tok = r / p.group, head = kvh * p.group + r % p.group;
-    if (r < work.tokens * p.group) {
-        const int64_t step = (D + 2) * kRows;
-        const float *sums = p.work + (tile - p.whole) * p.split * step + r;
-        float top = -INFINITY;
+    if (r >= work.tokens * p.group) return;
+    const int64_t step = (D + 2) * kRows;
+    const float *sums = p.work + (tile - p.whole) * p.split * step + r;
+    float top = -INFINITY;
 #pragma unroll 8
-        for (int i = 0; i < p.split; ++i) top = fmaxf(top, sums[i * step + D * kRows]);
-        const float z = top == -INFINITY ? 0.0f : top;
-        float l = 0.0f, o[8] = {};
-#pragma unroll 4
-        for (int i = 0; i < p.split; ++i) {
-            const float *part = sums + i * step, by = ex2(part[D * kRows] - z);
-            l += by * part[(D + 1) * kRows];
+    for (int i = 0; i < p.split; ++i) top = fmaxf(top, sums[i * step + D * kRows]);
+    const float z = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, o[8] = {};
+    for (int i0 = 0; i0 < p.split; i0 += kJoinParts) {
+        // the loads of some parts are all on their way before the first is used; no branch, behind which they would sink
+        float by[kJoinParts], x[kJoinParts][9];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] += by * part[(warp * 8 + e) * kRows];
+        for (int i = 0; i < kJoinParts; ++i) {
+            const bool on = i0 + i < p.split;
+            const float *part = sums + (on ? i0 + i : 0) * step;
+            by[i] = part[D * kRows], x[i][8] = part[(D + 1) * kRows];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = part[(warp * 8 + e) * kRows];
+            by[i] = on ? ex2(by[i] - z) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 9; ++e) x[i][e] = on ? x[i][e] : 0.0f;
         }
-        if (p.sinks) l += sink_weight(p.sinks[head], z);
-        const float by = top == -INFINITY ? 0.0f : 1.0f / l;
-        float worst = isnan(l) ? l : 0.0f;  // 0, or NaN
 #pragma unroll
-        for (int e = 0; e < 8; ++e) worst += o[e] * 0.0f, o[e] *= by;
-        store8<TYPE>(p.out.p + (int64_t)(work.tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + warp * 16, o);
-        if (worst != 0.0f) again[lane] = 1;
+        for (int i = 0; i < kJoinParts; ++i) {
+            l += by[i] * x[i][8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] += by[i] * x[i][e];
+        }
     }
-    __syncthreads();
-    if (warp == 0 && again[lane]) {
-        const int at = work.at0 + tok;
-        row_again<D, TYPE>(p, work.tok0 + tok, head, work.k0, p.window > 0 ? max(0, at - p.window + 1) : 0, at);
-    }
+    const bool none = top == -INFINITY && !isnan(l);
+    if (p.sinks) l += sink_weight(p.sinks[head], z);
+    const float by = none ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= by;
+    store8<TYPE>(p.out.p + (int64_t)(work.tok0 + tok) * p.out.ts + (int64_t)head * p.out.hs + warp * 16, o);
 }
 
 // [tokens][heads][D] rows as a 3-D map with boxes of 64 elements x heads x tokens.
@@ -783,7 +887,7 @@ int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, c
     if (device < 0 || device >= kMaxDevices) return reject("device ordinal out of range");
     if (q_tokens == 0) return AMOE_OK;
     PrefillParams p{};
-    p.q = rows_dev(q), p.k = rows_dev(k), p.v = rows_dev(v), p.out = rows_dev(out);
+    p.v = rows_dev(v), p.out = rows_dev(out);
     p.cu_q = cu_q, p.cu_k = cu_k;
     p.sinks = attn->sinks;
     p.scale_log2 = attn_scale(attn, head_dim) * kLog2e;

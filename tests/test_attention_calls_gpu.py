@@ -7,7 +7,8 @@ import torch
 
 import attention_ref as R
 from airllm_b200 import AmoeError, attention, moe
-from test_attention_gpu import BF16, E4M3, F16, F32, filled, gen, i32, on_gpu, randn, starts, table_for
+from test_attention_gpu import (BF16, E4M3, F16, F32, PREFILLS, SPLITS, filled, gen, i32, on_gpu, randn, starts,
+                                table_for)
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +168,80 @@ def test_append_rotates_by_the_published_frequencies(cuda_device, d, yarn):
     want = R.rotated(x[:, :5], pos, freq, conc).double()
     got = torch.cat((q, k_out), 1).cpu().double()
     assert ((got - want).abs() <= 2.0 ** -23 * want.abs() + far).all()
+
+
+# ---- values that are not finite ----------------------------------------------------------------
+@pytest.mark.parametrize("share", [0.003, 0.1, 1.0])
+@pytest.mark.parametrize("case", range(len(PREFILLS) + len(SPLITS)))
+def test_prefill_of_odd_values(cuda_device, case, share):
+    """Infinities and NaN strewn over V: an element is the formula's sum over the keys that its row sees, an infinity
+    of either sign and NaN included, and no row has anything of a key that it does not see."""
+    new, before, heads, kv, d, dtype, window, with_sinks = (PREFILLS + SPLITS)[case]
+    g = gen(600 + case)
+    keys = [a + b for a, b in zip(new, before)]
+    n, m = sum(new), sum(keys)
+    q, k, v = randn(g, n, heads, d, dtype=dtype, scale=0.5), randn(g, m, kv, d, dtype=dtype), randn(g, m, kv, d, dtype=dtype)
+    odd = torch.tensor([math.inf, -math.inf, math.nan, math.inf], dtype=dtype)
+    rows = torch.rand(m, kv, generator=g) < share
+    hit = rows[..., None] & (torch.rand(m, kv, d, generator=g) < (0.03 if share < 1 else 1.0))
+    v[hit] = odd[torch.randint(0, 4, (int(hit.sum()),), generator=g)]
+    sinks = randn(g, heads) if with_sinks else None
+    out = attention.prefill(q.cuda(), k.cuda(), v.cuda(), starts(new).cuda(), starts(keys).cuda(), window=window,
+                            sinks=None if sinks is None else sinks.cuda()).cpu().double()
+    some = sorted({0, heads // kv - 1, heads - 1})  # heads
+    a = b = 0
+    for x, y in zip(new, keys):
+        for h in some:
+            one = h * kv // heads
+            want, bound = R.attention(q[a:a + x, h:h + 1], k[b:b + y, one:one + 1], v[b:b + y, one:one + 1],
+                                      None if sinks is None else sinks[h:h + 1], window)
+            got, fine = out[a:a + x, h:h + 1], torch.isfinite(want)
+            assert torch.equal(torch.nan_to_num(got[~fine], 9.0, 7.0, 8.0), torch.nan_to_num(want[~fine], 9.0, 7.0, 8.0))
+            assert torch.isfinite(got[fine]).all() and ((got - want).abs()[fine] <= bound[fine]).all()
+        a, b = a + x, b + y
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F16, 128)])
+def test_an_infinity_does_not_make_prefill_slow(cuda_device, dtype, d):
+    """Computing rows again, key by key, took 60 to 360 times as long; three times leaves room for noise."""
+    n = 4096
+    q, k, v = (torch.randn(n, h, d, device="cuda").to(dtype) for h in (64, 8, 8))
+    cu = i32([0, n]).cuda()
+
+    def ms(values):
+        times = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            attention.prefill(q, k, values, cu)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return sorted(times)[2]
+
+    one, row = v.clone(), v.clone()
+    one[5, 0, 3], row[n // 2] = math.inf, math.nan
+    clean = ms(v)
+    for values in (one, row, torch.full_like(v, math.nan)):
+        assert ms(values) < 3 * clean
+
+
+@pytest.mark.parametrize("window", [1, 0])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F16, 64), (BF16, 128)])
+def test_prefill_scores_that_are_not_finite(cuda_device, dtype, d, bad, window):
+    """A score of NaN or +inf makes its row NaN, whichever column of a tile its key stands in and although the row sees
+    nothing else; a window of one key shows each column alone."""
+    g = gen(64)
+    n = 200
+    q, k, v = randn(g, n, 2, d, dtype=dtype), randn(g, n, 1, d, dtype=dtype), randn(g, n, 1, d, dtype=dtype)
+    q[:, :, 0] = 1.0
+    first = 64
+    k[first::2, 0, 0] = bad
+    out = attention.prefill(q.cuda(), k.cuda(), v.cuda(), i32([0, n]).cuda(), window=window).cpu()
+    hit = torch.arange(n) >= first
+    if window:
+        hit &= torch.arange(n) % 2 == 0
+    assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
+    if window:
+        assert torch.equal(out[~hit], v[~hit].expand(-1, 2, d))
