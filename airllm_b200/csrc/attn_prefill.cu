@@ -224,7 +224,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// 2^x of two values on the FMA pipe, to 2^-23: with n the integer next to x (read from the low bits of
+// 2^x of two values on the FMA pipe, to 2^-22.1: with n the integer next to x (read from the low bits of
 // x + 1.5 * 2^23) and f = x - n in [-1/2, 1/2], 2^f by a polynomial of degree 5 fitted to the least relative error,
 // and n added to its exponent.  Below -127 the result is a zero or the smallest subnormal, and so is it for NaN.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {

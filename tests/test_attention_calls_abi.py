@@ -2,8 +2,10 @@
 import ctypes
 import math
 import os
+import re
 import subprocess
 
+import numpy as np
 import pytest
 
 from airllm_b200 import AmoeError, attention, build, moe
@@ -133,3 +135,29 @@ def test_the_search_for_sequences(tmp_path):
                     "-o", exe, os.path.join(CUDA, "kv_search_check.cu")], check=True)
     got = subprocess.run([exe], capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout.strip() == "ok", got.stdout
+
+
+def test_the_polynomial_of_the_exponentials():
+    """2^x on the FMA pipe as attn_prefill.cu writes it, step by step in float32 (a product of two float32 is exact in
+    float64, so adding there and rounding once is a fused step but for double roundings), against 2^x in float64."""
+    src = open(os.path.join(build.CSRC, "attn_prefill.cu")).read()
+    body = src[src.index("float2 ex2_poly("):]
+    body = body[:body.index("\n}")]
+    coeff = [np.float32(a) for a, b in re.findall(r"pair\(([\d.]+)f, ([\d.]+)f\)", body) if a == b and float(a) < 2]
+    assert len(coeff) == 6
+    f32, f64 = np.float32, np.float64
+
+    def fma(a, b, c):
+        return (a.astype(f64) * f64(b) + f64(c) if np.isscalar(b) else a.astype(f64) * b.astype(f64) + f64(c)).astype(f32)
+
+    x = np.concatenate([np.linspace(-0.5, 0.5, 400001), np.linspace(-126, 16, 400001)]).astype(f32)
+    t = x + f32(12582912.0)
+    n = t - f32(12582912.0)
+    f = x - n  # exact
+    y = np.full_like(f, coeff[0])
+    for c in coeff[1:]:
+        y = fma(y, f, c)
+    got = (y.view(np.int32) + (t.view(np.uint32).astype(np.int64) << 23).astype(np.uint32).view(np.int32)).view(f32)
+    off = np.abs(got.astype(f64) / np.exp2(x.astype(f64)) - 1).max()
+    assert 2.0 ** -22.5 < off <= 2.0 ** -22.1  # the bound that the source states, and that it is not idle
+    assert "to 2^-22.1:" in src
