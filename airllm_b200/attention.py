@@ -34,6 +34,7 @@ from .moe import (AMOE_ERR_INVALID, AMOE_OK, GGUF_BF16, GGUF_F16, GGUF_F32, KV_B
                   KV_PAST_TABLE, AmoeError, AmoeKvCache, AmoeRope, load_library)
 
 _TYPES = {torch.float32: GGUF_F32, torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16}
+_LEAST, _MOST = 2.0 ** -149, torch.finfo(torch.float32).max
 _CACHE_TYPES = {torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16, torch.float8_e4m3fn: KV_E4M3}
 
 
@@ -119,8 +120,8 @@ def _empty(like, shape, dtype, stream):
 def _attn(scale, window: int, sinks, heads: int, device: int) -> bytes:
     if scale is None:
         scale = 0.0
-    elif not scale > 0:
-        _invalid("scale must be positive")
+    elif not _LEAST <= scale <= _MOST:  # float32 would make it 0, the default, or an infinity
+        _invalid("scale must be positive, finite and a float32")
     at = 0
     if sinks is not None:
         if sinks.dtype != torch.float32 or sinks.dim() != 1 or sinks.shape[0] != heads or not sinks.is_contiguous():

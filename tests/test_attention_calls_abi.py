@@ -3,6 +3,7 @@ import ctypes
 import math
 import os
 import re
+import struct
 import subprocess
 
 import numpy as np
@@ -161,3 +162,16 @@ def test_the_polynomial_of_the_exponentials():
     off = np.abs(got.astype(f64) / np.exp2(x.astype(f64)) - 1).max()
     assert 2.0 ** -22.5 < off <= 2.0 ** -22.1  # the bound that the source states, and that it is not idle
     assert "to 2^-22.1:" in src
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e39, math.inf, math.nan, 0.0, -1.0, -math.inf])
+def test_scales_that_float32_does_not_hold(scale):
+    """1e-50 became 0, which asks for the default; 1e39 raised something else."""
+    with pytest.raises(AmoeError, match="scale"):
+        attention._attn(scale, 0, None, 8, 0)
+
+
+def test_scales_that_float32_holds():
+    for scale in (2.0 ** -149, 0.125, 3e38):
+        assert struct.unpack("fiP", attention._attn(scale, 7, None, 8, 0))[0] == np.float32(scale)
+    assert struct.unpack("fiP", attention._attn(None, 7, None, 8, 0)) == (0.0, 7, 0)
