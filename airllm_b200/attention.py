@@ -329,6 +329,7 @@ class KVCache:
         if not bits:
             return
         self.status.zero_()
+        torch.cuda.synchronize(self.device)  # before a call on another stream reports anew
         said = [m for b, m in ((KV_BAD_PAGE, "a page id outside the cache"),
                                (KV_PAST_TABLE, "a position beyond the page table"),
                                (KV_BAD_LENGTHS, "negative or decreasing lengths")) if bits & b]

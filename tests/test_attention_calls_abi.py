@@ -175,3 +175,24 @@ def test_scales_that_float32_holds():
     for scale in (2.0 ** -149, 0.125, 3e38):
         assert struct.unpack("fiP", attention._attn(scale, 7, None, 8, 0))[0] == np.float32(scale)
     assert struct.unpack("fiP", attention._attn(None, 7, None, 8, 0)) == (0.0, 7, 0)
+
+
+def test_check_clears_the_status_before_it_returns(monkeypatch):
+    """The report is cleared on the current stream; a call on another stream may follow at once, and what it reports must
+    not be cleared with it."""
+    log = []
+
+    class Status:
+        def item(self):
+            log.append("read")
+            return moe.KV_BAD_PAGE
+
+        def zero_(self):
+            log.append("clear")
+
+    cache = attention.KVCache.__new__(attention.KVCache)
+    cache.status, cache.device = Status(), "cuda:0"
+    monkeypatch.setattr(attention.torch.cuda, "synchronize", lambda device=None: log.append("wait"))
+    with pytest.raises(AmoeError, match="page id"):
+        cache.check()
+    assert log == ["wait", "read", "clear", "wait"]
