@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D, CACHE>::kCtas - (NB == 2 && 
             // the keys from `from` to `end` of this tile
             live = FULL;
             if (at < from) live &= FULL << (from - at);
-            if (at + KEYS > end) live &= FULL >> (at + KEYS - end);
+            if ((uint32_t)at + KEYS > (uint32_t)end) live &= FULL >> ((uint32_t)at + KEYS - end);  // may pass 2^31
             if (page < 0) live = 0;
             const uint32_t first = page >= 0 ? (uint32_t)cache_row(p.c, page, kvh, at) : 0u;
             row = first + lane % KEYS;

@@ -245,3 +245,27 @@ def test_prefill_scores_that_are_not_finite(cuda_device, dtype, d, bad, window):
     assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
     if window:
         assert torch.equal(out[~hit], v[~hit].expand(-1, 2, d))
+
+
+# ---- far positions -----------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,d,page", [(BF16, 64, 4096), (E4M3, 64, 4096), (F16, 128, 1024), (BF16, 64, 16)])
+@pytest.mark.parametrize("short", [0, 1, 17])
+def test_decode_next_to_2_31(cuda_device, kind, d, page, short):
+    """The last positions that a length can name, over a table that repeats a few pages: a window's keys, and not the slot
+    behind the last."""
+    g = gen(81)
+    n, window, kv = 2 ** 31 - 1 - short, 70, 1
+    pages = filled(g, 3, kv, page, d, kind)
+    cache = on_gpu(pages)
+    width = 2 ** 31 // page if page >= 1024 else 2 ** 27
+    table = torch.zeros(1, width, dtype=torch.int32)
+    table[0, -1], table[0, -2] = 2, 1
+    last = torch.full((1,), n, dtype=torch.int32)
+    q = randn(g, 1, 4, d, dtype=BF16 if kind == E4M3 else kind)
+    got = cache.decode(q.cuda(), table.cuda(), last.cuda(), window=window, max_len=1000)
+    cache.check()
+    pos = torch.arange(n - window, n)
+    ids, slot = table[0, pos // page].long(), pos % page
+    k, v = (R.values(c.view(torch.uint8)[ids, :, slot].view(c.dtype) if s is not None else c[ids, :, slot],
+                     None if s is None else s[ids, :, slot]) for c, s in pages)
+    R.close(got, *R.attention(q, k, v))
