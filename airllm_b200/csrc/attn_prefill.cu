@@ -253,9 +253,9 @@ __device__ __forceinline__ bool find_work(const PrefillParams &p, int x, int par
         const int s = s0 + lane;
         int a = 0, b = 0, k0 = 0, k1 = 0, tiles = 0;
         if (s < p.seqs) {
-            a = p.cu_q[s], b = min(p.cu_q[s + 1], p.q_tokens);
+            a = max(p.cu_q[s], 0), b = min(p.cu_q[s + 1], p.q_tokens);
             k0 = max(p.cu_k[s], 0), k1 = min(p.cu_k[s + 1], p.k_tokens);
-            if (a >= 0 && a < b) tiles = (b - a - 1) / p.tile_tokens + 1;
+            if (a < b) tiles = (b - a - 1) / p.tile_tokens + 1;
         }
         int upto = tiles;
 #pragma unroll

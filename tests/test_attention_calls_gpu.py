@@ -269,3 +269,15 @@ def test_decode_next_to_2_31(cuda_device, kind, d, page, short):
     k, v = (R.values(c.view(torch.uint8)[ids, :, slot].view(c.dtype) if s is not None else c[ids, :, slot],
                      None if s is None else s[ids, :, slot]) for c, s in pages)
     R.close(got, *R.attention(q, k, v))
+
+
+def test_prefill_clamps_starts(cuda_device):
+    """A first start below zero is the first row, one behind the rows given their end; the rows are written all the same."""
+    g = gen(82)
+    n = 60
+    q, k, v = (randn(g, n, 4, 64, dtype=BF16).cuda() for _ in range(3))
+    want = attention.prefill(q, k, v, i32([0, 25, n]).cuda())
+    for cu_q, cu_k in (([-4, 25, n], [0, 25, n]), ([-(1 << 31), 25, 2 ** 31 - 1], [-7, 25, n + 9])):
+        out = torch.full_like(q, 7.0)
+        attention.prefill(q, k, v, i32(cu_q).cuda(), i32(cu_k).cuda(), out=out)
+        assert torch.equal(out, want)
