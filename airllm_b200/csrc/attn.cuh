@@ -101,6 +101,11 @@ __device__ __forceinline__ int page_of(const CacheDev &c, int s, int64_t pos) {
     return page;
 }
 
+// The last of `fills` fills (the i-th goes to stage i % stages) that went to this stage; -1: none did.
+__host__ __device__ inline int last_fill(int fills, int stage, int stages) {
+    return fills > stage ? (fills - 1 - stage) / stages * stages + stage : -1;
+}
+
 // Row index of (page, head, slot) in the pages.
 __host__ __device__ inline int64_t cache_row(const CacheDev &c, int page, int head, int64_t pos) {
     return ((((int64_t)page * c.heads + head) << c.shift) | (pos & ((1 << c.shift) - 1)));

@@ -411,6 +411,7 @@ __device__ __forceinline__ bool tile_pass(const PrefillParams &p, const CUtensor
         const uint64_t q_d = desc_sw128(smem_u32(q_s), 16), k_d = desc_sw128(smem_u32(k_s), 16);
         const uint64_t v_d = desc_sw128(smem_u32(v_s), N * 128);
         bool ok = tiles > 0 && (CAREFUL || wait_warp(q_full, 0, work));
+        int scored = 0, weighed = 0;  // tiles whose products are issued
         auto scores = [&](int j) {  // S = Q K^T of tile j
             if (j >= tiles) return;
             const int s = j % kStages;
@@ -428,6 +429,7 @@ __device__ __forceinline__ bool tile_pass(const PrefillParams &p, const CUtensor
                 if (j > 0 && j - 1 + kStages < tiles) load(k_s, tm_k, k_full, j - 1 + kStages);
             }
             __syncwarp();
+            scored = j + 1;
         };
         auto weigh = [&](int t) {  // O += P V of tile t
             if (t < 0 || !ok) return;
@@ -480,11 +482,24 @@ __device__ __forceinline__ bool tile_pass(const PrefillParams &p, const CUtensor
                 if (t > 0 && t - 1 + kStages < tiles) load(v_s, tm_v, v_full, t - 1 + kStages);
             }
             __syncwarp();
+            weighed = t + 1;
         };
         for (int j = 0; ok && j <= tiles; ++j) {
             scores(j);
             weigh(j - 1);
         }
+        // Whatever gave up, nothing of the CTA's is in flight when it ends (its successor's memory would get it): the products,
+        // then the last copy to each stage, waited for without a look at work->dead, a second each at most.
+        if (scored > 0) bs::mbar_wait(s_full, (uint32_t)(scored - 1) & 1u, &work->dead, 1);
+        if (weighed > 0) bs::mbar_wait(o_done, (uint32_t)(weighed - 1) & 1u, &work->dead, 1);
+        if (tiles > 0 && !CAREFUL) bs::mbar_wait(q_full, 0, &work->dead, 1);
+        for (int s = 0; s < kStages; ++s) {
+            const int k = last_fill(min(max(scored - 1, 0) + kStages, tiles), s, kStages);
+            const int v = last_fill(min(max(weighed - 1, 0) + kStages, tiles), s, kStages);
+            if (k >= 0) bs::mbar_wait(k_full + s, (uint32_t)(k / kStages) & 1u, &work->dead, 1);
+            if (v >= 0) bs::mbar_wait(v_full + s, (uint32_t)(v / kStages) & 1u, &work->dead, 1);
+        }
+        __syncwarp();
         if (CAREFUL) asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");  // work->odd is as it stays
     } else {
         // a thread's row: token r / group of the tile, query head r % group of the kv head

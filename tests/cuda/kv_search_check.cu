@@ -1,5 +1,6 @@
 // Host-side check of the search for packed rows' sequences (attn.cuh: find_seqs), the one that the kernels run, over
 // more sequences than a warp looks at in one step: right for starts that ascend, in range for any others.
+// And the last fill of a ring's stage, which the prefill waits for before it ends.
 // Prints "ok" or the first case that fails.
 #include "attn.cuh"
 
@@ -36,5 +37,13 @@ int main() {
                 return printf("row %d of %d sequences not in %d\n", t + k, seqs, s), 1;
         }
     }
+    for (int stages = 1; stages < 5; ++stages)
+        for (int fills = 0; fills < 20; ++fills)
+            for (int s = 0; s < stages; ++s) {
+                int want = -1;
+                for (int i = 0; i < fills; ++i)
+                    if (i % stages == s) want = i;
+                if (last_fill(fills, s, stages) != want) return printf("last fill of stage %d of %d\n", s, stages), 1;
+            }
     return printf("ok\n"), 0;
 }
