@@ -271,6 +271,8 @@ class KVCache:
         """Sequence s's keys and values from position first[s] (default 0) on as packed rows
         cu[s]..cu[s+1] (amoe_kv_read).  Returns (k, v) [total, kv_heads, head_dim]: k_out and v_out,
         or new tensors of ``dtype`` (default: the cache's own type, bfloat16 for E4M3)."""
+        if total < 0:
+            _invalid("total must not be negative")
         d, dev = self.head_dim, self._index
         seqs, count = self._seqs(page_table)
         raw, st = _stream(stream, dev)

@@ -281,3 +281,10 @@ def test_prefill_clamps_starts(cuda_device):
         out = torch.full_like(q, 7.0)
         attention.prefill(q, k, v, i32(cu_q).cuda(), i32(cu_k).cuda(), out=out)
         assert torch.equal(out, want)
+
+
+def test_refusals_raise_the_library_error(cuda_device):
+    cache = attention.KVCache(4, 16, 2, 64)
+    table, cu = i32([[0, 1]]).cuda(), i32([0, 5]).cuda()
+    with pytest.raises(AmoeError, match="total"):
+        cache.read(table, cu, -1)
