@@ -21,7 +21,8 @@ nothing waits for it.  Inputs, outputs and the cache must be ready on that strea
 any torch operation.  Rows may be strided views with adjacent elements whose strides and
 address are multiples of 16 bytes (a fused projection's slices are).  Arguments that cannot
 be served raise ``AmoeError``; wrong page ids and lengths, which only the device sees, are
-skipped there and reported by ``KVCache.check``.
+skipped there and reported by ``KVCache.check``.  Rows that a call writes must not lie in its inputs'
+memory.  The operators serve; they have no backward pass, and their results carry no gradient.
 """
 from __future__ import annotations
 

@@ -26,11 +26,11 @@
 //
 // E4M3 keys and values meet f16 operands (every code is an f16 value).  A key's scale multiplies
 // its score.  A value's scale 2^e goes into the weight: w = exp2(t + e - m), t the score in
-// log2 and m the running maximum of t + e, so the 16-bit weight keeps its precision whatever
-// the scales are; the denominator sums exp2(t - n) with a maximum n of its own.
+// log2 and m the running maximum of t + e, so that what a weight may lose is small beside the largest product
+// whatever the scales are; the denominator sums exp2(t - n) with a maximum n of its own.
 //
-// Measured (B200): 131072 tokens, 8 kv heads, f16: 49.2 us, 5.5 TB/s, 0.83 of the copy bandwidth.
-// 48 sequences of 4096-8192 tokens, E4M3: 70 us, 4.3 TB/s, 0.66: the ALU pipe is 44 % busy (the codes'
+// Measured (B200): 131072 tokens, 8 kv heads, f16: 47.6 us in a graph, 5.6 TB/s, 0.86 of the copy bandwidth; 49.6 call after call.
+// 48 sequences of 4096-8192 tokens, E4M3: 70 us, 4.3 TB/s, 0.65: the ALU pipe is 50 % busy (the codes'
 // conversions) and sequences of unequal lengths leave SMs idle at the end.  E4M3 products (m16n8k32, queries
 // and weights as two E4M3 terms each) took 89 us.
 #include "attn.cuh"

@@ -16,11 +16,12 @@
 //
 // What bounds it.  64-wide heads: the exponentials, one a score on a pipe of 16 a clock an SM; 128 x 64 scores take 512
 // clocks there and 256 on the tensor cores.  Measured in steady state: 600 clocks a tile; 8192 tokens of 64 heads over
-// 8: 704 us, 780 TFLOP/s, 0.47 of the measured bf16 GEMM.  Two row tiles of one persistent CTA (0.93 ms: fewer warps
+// 8: 687 us in short runs, 800 TFLOP/s, 0.49 of the measured bf16 GEMM; 763 us and 720 TFLOP/s call after call, when
+// the power cap lowers the clock (0.52 of the GEMM's sustained rate).  Two row tiles of one persistent CTA (0.93 ms: fewer warps
 // to hide a tile's chain of waits), two threads a row (0.85 ms: the pair has to agree on its maximum) and P in S's
 // own columns (0.80 ms: Q K^T waits for P V) were slower.  128-wide heads: the tensor cores and the operands they read
-// from shared memory; 1500 tokens in three chunks behind 2600-2800 each: 87 us, 835 TFLOP/s.  Windows and short
-// prompts: a CTA's start.
+// from shared memory; 1500 tokens in three chunks behind 2600-2800 each: 90 to 95 us in a graph, 100 a call (730 TFLOP/s).
+// Windows and short prompts: a CTA's start.
 //
 // A few queries behind many keys, or the last wave of a larger call, do not fill the GPU: the keys of those tiles are
 // split over CTAs, and a second kernel joins the partial sums (`layout` below chooses, with what it measured).
@@ -834,8 +835,8 @@ struct Layout {
 // split.  The split is the one of the least expected time: a CTA takes 1 us for 64 keys however many share its SM, and
 // 4 us to start and end; the join takes 3 us, 1/4 us a part that its threads walk, and the partial sums' way through
 // L2 15 ns (64-wide heads) or 30 ns a CTA.  Measured, one CTA a tile -> split (64/8 heads of 64): 16 queries behind
-// 2048 keys 29 -> 12.6 us in 8 parts (14.4 in 16), behind 32768 460 -> 37 us in 32; 512 behind 8192 129 -> 120 us in 3;
-// 128 behind none 6.0 us, in 2 parts 8.9.  32/8 heads of 128: 64 behind 8192 134 -> 31 us; 300 behind 3000 55 -> 32 us
+// 2048 keys 29 -> 12 us in 8 parts (14.4 in 16), behind 32768 460 -> 34 us in 32; 512 behind 8192 129 -> 122 us in 3;
+// 128 behind none 6.0 us, in 2 parts 8.9.  32/8 heads of 128: 64 behind 8192 134 -> 26 us; 300 behind 3000 55 -> 32 us
 // in 3 (39 in 4); 1500 behind 8000 (296 whole tiles, 80 split) 256 -> 206 us in 3 (216 in 4; all tiles in 3: 233); 1400
 // behind none 27.5 us, its last tiles in 2 parts 33.
 constexpr int kMaxSplit = 32;

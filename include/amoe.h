@@ -335,7 +335,8 @@ typedef struct amoe_rows {
 enum { AMOE_KV_E4M3 = 100 };
 
 /* What kernels add to *status when a page table or length is wrong; the rows concerned are
- * not written (append), read as zeros (read) or not seen (decode). */
+ * not written (append), read as zeros (read) or not seen (decode).  Append and read look at all of
+ * a call's starts, those of sequences without a row given too. */
 enum {
     AMOE_KV_BAD_PAGE = 1,    /* a page id outside [0, pages) */
     AMOE_KV_PAST_TABLE = 2,  /* a position beyond table_stride * page_size */
@@ -427,7 +428,8 @@ typedef struct amoe_attn {
  * such as a CUDA tensor map takes.  workspace: amoe_attn_prefill_workspace's bytes of device
  * memory (NULL where that is 0), 16-byte aligned, the call's own until it has run; its
  * contents before and after mean nothing.  A wait inside the kernel that gives up after about a
- * second leaves NaN rows, or rows that took long. */
+ * second leaves NaN rows.  Infinities and NaN in v that a query sees come out as the sum has them, in
+ * about twice the time at most. */
 AMOE_API int amoe_attn_prefill(int32_t device, int32_t head_dim, const amoe_attn *attn, const amoe_rows *q,
                                const amoe_rows *k, const amoe_rows *v, const amoe_rows *out, int32_t q_tokens,
                                int32_t k_tokens, const int32_t *cu_q, const int32_t *cu_k, int32_t seqs,
