@@ -162,8 +162,11 @@ class Rope:
 
     def _new(self):
         self._c = AmoeRope()
-        self._at = ctypes.addressof(self._c)
         return load_library()
+
+    @property
+    def _at(self) -> int:  # not kept: a copied Rope has a table of its own
+        return ctypes.addressof(self._c)
 
     @property
     def frequencies(self) -> list:

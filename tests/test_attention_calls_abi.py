@@ -1,4 +1,5 @@
 """Calls of the attention entry points that the documentation allows, on the host side (no GPU)."""
+import copy
 import ctypes
 import math
 import os
@@ -196,3 +197,12 @@ def test_check_clears_the_status_before_it_returns(monkeypatch):
     with pytest.raises(AmoeError, match="page id"):
         cache.check()
     assert log == ["wait", "read", "clear", "wait"]
+
+
+def test_a_copied_rope_has_its_own_table():
+    """A deep copy kept the address of the original's table, which ends with the original."""
+    rope = attention.Rope.yarn(64, 150000.0)
+    other = copy.deepcopy(rope)
+    rope._c.freq[0] = 7.0
+    assert other.frequencies[0] == 1.0
+    assert other._at == ctypes.addressof(other._c) != rope._at
