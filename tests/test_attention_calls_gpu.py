@@ -203,7 +203,7 @@ def test_prefill_of_odd_values(cuda_device, case, share):
 
 @pytest.mark.parametrize("dtype,d", [(BF16, 64), (F16, 128)])
 def test_an_infinity_does_not_make_prefill_slow(cuda_device, dtype, d):
-    """Computing rows again, key by key, took 60 to 360 times as long; three times leaves room for noise."""
+    """Computing rows again, key by key, took 60 to 360 times as long."""
     n = 4096
     q, k, v = (torch.randn(n, h, d, device="cuda").to(dtype) for h in (64, 8, 8))
     cu = i32([0, n]).cuda()
@@ -223,7 +223,7 @@ def test_an_infinity_does_not_make_prefill_slow(cuda_device, dtype, d):
     one[5, 0, 3], row[n // 2] = math.inf, math.nan
     clean = ms(v)
     for values in (one, row, torch.full_like(v, math.nan)):
-        assert ms(values) < 3 * clean
+        assert ms(values) < 10 * clean  # 2.2 measured
 
 
 @pytest.mark.parametrize("window", [1, 0])
