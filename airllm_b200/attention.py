@@ -17,8 +17,8 @@ rope.go:10-86).  A serving loop holds one ``KVCache`` a layer, all over one page
     out = cache.decode(q, table, length + 1, window=128, sinks=sinks)
 
 Work is enqueued on ``stream`` (default: torch's current stream on the tensors' device) and
-nothing waits for it.  Inputs, outputs and the cache must be ready on that stream, as with
-any torch operation.  Rows may be strided views with adjacent elements whose strides and
+nothing waits for it.  Inputs, outputs and the cache must be ready on that stream, and not
+be freed before it has run them (``Tensor.record_stream``), as with any torch operation.  Rows may be strided views with adjacent elements whose strides and
 address are multiples of 16 bytes (a fused projection's slices are).  Arguments that cannot
 be served raise ``AmoeError``; wrong page ids and lengths, which only the device sees, are
 skipped there and reported by ``KVCache.check``.  Rows that a call writes must not lie in its inputs'
